@@ -103,7 +103,8 @@ int snb200_get_math_mode(snb200_handle_t handle, int* math_mode);
 /* Text of the last error recorded on this handle (never NULL; empty when none). */
 const char* snb200_last_error_string(snb200_handle_t handle);
 /* Waits for the handle's stream and returns EXECUTION_FAILED if a kernel reported a
- * device-side pipeline time-out since the last check. */
+ * device-side pipeline time-out since the last check, INVALID_VALUE if an embedding call met a token index outside
+ * its table. */
 int snb200_check_device_status(snb200_handle_t handle);
 /* Runs the failure path of the tensor-core kernels on purpose, harmlessly (no counterpart in SharpNet): one small
  * kernel waits on a barrier that nothing signals, with a limit of limit_us microseconds (1 .. 100000) instead of
@@ -359,6 +360,95 @@ int snb200_sgd_update(snb200_handle_t handle, long long count, float learning_ra
 int snb200_adam_update(snb200_handle_t handle, long long count, double learning_rate, double beta1, double beta2,
                        double epsilon, double weight_decay, int time_step, const float* dW, float* W, float* adam_vW,
                        float* adam_sW);
+
+/* The same Adam / AdamW update for ALL tensors of a model in one launch (up to 448 tensors per launch): what the loop
+ * of Network.UpdateWeights over the layers' Adam.UpdateWeights (Prod/Optimizers/Adam.cs:59-72) issues tensor by tensor.
+ * Element for element the formula of snb200_adam_update (last bits may differ), with weight_decay * decay of the tensor in place of
+ * weight_decay (decay 0 for biases and norms is customary).
+ * state_bits 32: adam_vW and adam_sW are float arrays of `count` elements; the scales are not read.
+ * state_bits 8: they are byte arrays of `count` elements, and v_scale and s_scale hold one float per 256 consecutive
+ *   elements, ceil(count / 256) each.  An element's v is its e4m3 code times its v_scale, its s the SQUARE of its code
+ *   times its s_scale.  All bytes zero is the state before the first step.  The scales are powers of two that bring the
+ *   block's largest magnitude to [128, 256); a block whose largest magnitude is below 2^-100 is held as zeros.  v is
+ *   rounded to nearest, the root of s up or down at random in proportion, from a hash of rounding_seed, the tensor's
+ *   place in the list and the element's (nearest rounding would hold an average that moves by a thousandth a step where
+ *   it is).  W is updated from the moments before they are rounded.  The same arguments give the same bits; pass another
+ *   rounding_seed every step (the time step itself will do).  A block that meets an infinite or NaN gradient is NaN from
+ *   then on.
+ * Tensors with count 0 are skipped.  The table is read during the call and not kept.  W, moments and scales of different
+ * tensors must not share memory (INVALID_VALUE).  A captured call replays with the step, rates and seed of its capture. */
+typedef struct snb200_adam_tensor {
+  long long count;
+  const float* dW;
+  float* W;
+  void *adam_vW, *adam_sW;
+  float *v_scale, *s_scale;   /* NULL for state_bits 32 */
+  double decay;
+} snb200_adam_tensor;
+int snb200_adam_group_update(snb200_handle_t handle, int n, const snb200_adam_tensor* tensors, int state_bits,
+                             double learning_rate, double beta1, double beta2, double epsilon, double weight_decay,
+                             int time_step, unsigned int rounding_seed);
+
+/* ---- embedding ----------------------------------------------------------------------------------
+ * y[t, :] = scale * table[indices[t], :] for t in [0, tokens), table [vocabulary, dim], y [tokens, dim].
+ * Replaces Tensor.WordEmbeddingForwardPropagation on dense inputs (NVRTC kernel WordEmbeddingForwardPropagation,
+ * Prod/GPU/Kernels/SinglePrecision.cu:617).  The indices are int, long long, or floats as SharpNet's own tensors hold
+ * them (rounded to the nearest integer), aligned to their type.  A row whose index lies outside the table (a NaN counts
+ * as outside) is written as zeros, and the next snb200_check_device_status returns INVALID_VALUE once. */
+enum { SNB200_INDEX_INT32 = 0, SNB200_INDEX_INT64 = 1, SNB200_INDEX_FP32 = 2 };
+int snb200_embedding_fwd(snb200_handle_t handle, int index_type, long long tokens, int vocabulary, int dim,
+                         const void* indices, float scale, const float* table, float* y);
+/* dtable[v, :] = (accumulate ? dtable[v, :] : 0) + scale * sum over the tokens t with indices[t] == v of dy[t, :].
+ * Replaces Tensor.WordEmbeddingBackwardPropagation (SinglePrecision.cu:650, atomicAdd): the tokens are sorted by word
+ * and each word's rows are added in the order of their tokens, so the same call gives the same bits.  Tokens with index
+ * padding_index (-1: none) and tokens whose index lies outside the table contribute nothing; the latter are reported
+ * like those of the forward call.  With accumulate, rows of words that do not occur are left as they are.
+ * `scratch` is caller-provided device memory of at least snb200_embedding_scratch_bytes(tokens, vocabulary, dim) bytes,
+ * 16-byte aligned (-1: invalid sizes); calls that may run at the same time need one each.  At most 2^30 tokens. */
+long long snb200_embedding_scratch_bytes(long long tokens, int vocabulary, int dim);
+int snb200_embedding_bwd(snb200_handle_t handle, int index_type, long long tokens, int vocabulary, int dim,
+                         const void* indices, float scale, int padding_index, int accumulate, const float* dy,
+                         void* scratch, float* dtable);
+
+/* ---- norm, gate and residual between two blocks ---------------------------------------------------
+ * One pass over the rows of x and of a block's output ("block", [rows, dim] both):
+ *   u = post_norm(block) ;  r = residual_scale * x + block_scale * gate * u ;  y = norm(r)
+ * where a norm is NONE (the identity; for `norm`: no y), LAYER ((t - mean) / sqrt(variance + epsilon) * gamma + beta) or
+ * RMS (t / sqrt(mean square + epsilon) * gamma + beta), over each row.  Replaces, together with SharpNet's AddLayer, the
+ * LayerNorm and RMSNorm kernels (Prod/GPU/Kernels/SinglePrecision.cu:32-297,1345).
+ *   gamma, beta, post_gamma, post_beta [dim]: NULL for 1 and 0;
+ *   gate [gate_rows, dim]: row i of the batch uses row i / (rows / gate_rows); gate_rows must divide rows (1: a gate per
+ *     channel; the batch size: one per sequence; rows: one per element); gate_rows 0 and gate NULL: no gate;
+ *   block NULL: r = residual_scale * x (a norm alone).  r may then be NULL if it is not needed, and may be x itself
+ *     whether or not there is a block;
+ *   stats, post_stats [rows, 2]: mean (0 for RMS) and 1 / deviation of each row for the backward pass, NULL if unwanted.
+ * epsilon must be above 0. */
+enum { SNB200_NORM_NONE = 0, SNB200_NORM_LAYER = 1, SNB200_NORM_RMS = 2 };
+typedef struct snb200_norm_desc {
+  long long rows;
+  int dim, norm, post_norm, gate_rows;
+  float residual_scale, block_scale, epsilon;
+} snb200_norm_desc;
+typedef struct snb200_norm_params {
+  const float *gamma, *beta, *post_gamma, *post_beta, *gate;
+} snb200_norm_params;
+typedef struct snb200_norm_gradients {
+  float *gamma, *beta, *post_gamma, *post_beta, *gate;      /* NULL where not wanted */
+} snb200_norm_gradients;
+int snb200_residual_norm_fwd(snb200_handle_t handle, const snb200_norm_desc* desc, const snb200_norm_params* params,
+                             const float* x, const float* block, float* r, float* y, float* stats, float* post_stats);
+/* The gradients from dy (of y; not read when norm is NONE) and dr (what reaches r past y; NULL for none):
+ *   dR = dr + norm'(dy) ;  dx = residual_scale * dR ;  dblock = post_norm'(block_scale * gate * dR)
+ * and the sums over the rows for the parameters (the gate's over the rows that share a row of it).  r, block, stats and
+ * post_stats are those of the forward pass (r: x itself when there was no block and residual_scale is 1; block is read
+ * only for post_norm and for the gradient of the gate).  Every output may be NULL, not all of them; dx may be dr.
+ * `scratch`: at least snb200_residual_norm_scratch_floats(desc) floats, 16-byte aligned; calls that may run at the same
+ * time need one each.  Sums are taken in a fixed order: the same call gives the same bits. */
+long long snb200_residual_norm_scratch_floats(const snb200_norm_desc* desc);
+int snb200_residual_norm_bwd(snb200_handle_t handle, const snb200_norm_desc* desc, const snb200_norm_params* params,
+                             const float* r, const float* block, const float* dy, const float* dr, const float* stats,
+                             const float* post_stats, float* scratch, float* dx, float* dblock,
+                             const snb200_norm_gradients* gradients);
 
 /* ---- data-parallel gradient sum -------------------------------------------------------------
  * Sum of the per-replica dW/db buffers, left on every replica.  Replaces the

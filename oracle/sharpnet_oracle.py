@@ -361,6 +361,166 @@ def update_adam_optimizer(W, learning_rate, beta1, beta2, epsilon, weight_decay,
 
 
 # --------------------------------------------------------------------------------------------
+# Adam over many tensors with 8-bit moments: the state bit for bit, in numpy's 32-bit arithmetic
+# --------------------------------------------------------------------------------------------
+def e4m3_decode(codes):
+    """The value of 8-bit floats with 4 bits of exponent (bias 7) and 3 of mantissa; 0x7f / 0xff are NaN."""
+    c = np.asarray(codes, np.uint8).astype(np.int64)
+    e, m = (c >> 3) & 15, c & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    v = np.where((c & 127) == 127, np.nan, v)
+    return np.where(c >= 128, -v, v)
+
+
+def e4m3_encode(x):
+    """Nearest code, ties to even, of finite values of magnitude up to 448: by search among all codes."""
+    table = e4m3_decode(np.arange(127, dtype=np.uint8))                   # 0 .. 448, ascending
+    a = np.abs(np.asarray(x, np.float64))
+    hi = np.clip(np.searchsorted(table, a), 1, 126)
+    lo = hi - 1
+    middle = (table[lo] + table[hi]) / 2
+    code = np.where(a > middle, hi, np.where(a < middle, lo, np.where(lo % 2 == 0, lo, hi)))
+    return (code + np.where(np.signbit(x), 128, 0)).astype(np.uint8)
+
+
+def adam8_scale(block_max):
+    """Power of two that brings the largest magnitude of a block to [128, 256); 0 below 2^-100, NaN where not finite."""
+    out = np.zeros(len(block_max), np.float32)
+    for i, m in enumerate(np.asarray(block_max, np.float32)):
+        if not np.isfinite(m):
+            out[i] = np.nan
+        elif m >= 2.0 ** -100:
+            out[i] = 2.0 ** (math.frexp(float(m))[1] - 8)
+    return out
+
+
+def adam8_random20(seed, ordinal, count):
+    """20 random bits for each of the first ``count`` elements of tensor ``ordinal``."""
+    m = 0xFFFFFFFF
+    pair = np.arange((count + 1) // 2, dtype=np.uint64)
+    x = (pair + np.uint64((seed * 0x9E3779B1 + ordinal * 0x85EB9A77) & m)) & np.uint64(m)
+    x = ((x ^ (x >> np.uint64(16))) * np.uint64(0x6C8E9CF5)) & np.uint64(m)
+    x = ((x ^ (x >> np.uint64(12))) * np.uint64(0xB5297A4D)) & np.uint64(m)
+    x = x ^ (x >> np.uint64(15))
+    both = np.stack(((x & np.uint64(0xFFFF)) << np.uint64(4), (x >> np.uint64(16)) << np.uint64(4)), 1)
+    return both.reshape(-1)[:count].astype(np.int64)
+
+
+def update_adam8_optimizer(W, learning_rate, beta1, beta2, epsilon, weight_decay, dW, v, s, v_scale, s_scale, time_step,
+                           seed, ordinal):
+    """In place.  W in float64 from the unrounded moments; the codes and scales exactly: each operation on the moments is
+    one 32-bit operation."""
+    f32 = np.float32
+    with np.errstate(all="ignore"):
+        n = W.size
+        blocks = -(-n // 256)
+        pad = lambda a: np.pad(a, (0, blocks * 256 - n)).reshape(blocks, 256)  # noqa: E731
+        b1, b2, g = f32(beta1), f32(beta2), pad(dW.reshape(-1))
+        vv = pad(e4m3_decode(v).astype(f32)) * v_scale[:, None]
+        r = pad(e4m3_decode(s).astype(f32)) * s_scale[:, None]
+        vv = b1 * vv + (f32(1) - b1) * g
+        sq = b2 * (r * r) + ((f32(1) - b2) * g) * g
+        root = np.sqrt(sq)
+        factor = learning_rate * (math.sqrt(1.0 - beta2 ** time_step) / (1.0 - beta1 ** time_step))
+        w = W.reshape(-1).astype(np.float64)
+        step = (factor * vv.astype(np.float64) / (root.astype(np.float64) + epsilon)).reshape(-1)[:n]
+        new_w = w - (step + weight_decay * w)
+        v_scale[...], s_scale[...] = adam8_scale(np.abs(vv).max(1)), adam8_scale(root.max(1))
+        inverse = [np.where(c == 0, f32(0), f32(1) / c)[:, None].astype(f32) for c in (v_scale, s_scale)]
+        finite = [np.isfinite(c) for c in (v_scale, s_scale)]
+        v[...] = e4m3_encode(np.where(finite[0][:, None], vv * inverse[0], f32(0)).reshape(-1)[:n])
+        x = np.where(finite[1][:, None], root * inverse[1], f32(0)).reshape(-1)[:n].astype(f32)
+        rnd = adam8_random20(seed, ordinal, n)
+        high = ((x.view(np.int32).astype(np.int64) + rnd) & ~0xFFFFF).astype(np.int32).view(f32)
+        low = np.maximum(np.floor(x * f32(512) + rnd.astype(f32) * f32(2.0 ** -20)), 1) * f32(2.0 ** -9)
+        s[...] = e4m3_encode(np.where(x < f32(2.0 ** -6), np.where(x > 0, low, f32(0)), high))
+    return new_w.reshape(W.shape)
+
+
+# --------------------------------------------------------------------------------------------
+# Word embedding (Prod/GPU/Kernels/SinglePrecision.cu:617,650), in float64
+# --------------------------------------------------------------------------------------------
+def embedding_forward(indices, scale, table):
+    """Indices outside the table give rows of zeros."""
+    ids = np.asarray(indices)
+    bad = ~((ids >= 0) & (ids < table.shape[0]))
+    ids = np.where(bad, 0, ids).astype(np.int64)
+    return np.where(bad[:, None], 0.0, scale * table[ids].astype(np.float64))
+
+
+def embedding_backward(indices, scale, padding_index, dy, dtable, accumulate):
+    """(gradient, sum of the magnitudes added, number of terms) by word."""
+    ids = np.asarray(indices)
+    keep = (ids >= 0) & (ids < dtable.shape[0]) & (ids != padding_index)
+    ids = np.where(keep, ids, 0).astype(np.int64)[keep]
+    total, size = np.zeros(dtable.shape), np.zeros(dtable.shape)
+    np.add.at(total, ids, scale * dy[keep].astype(np.float64))
+    np.add.at(size, ids, np.abs(scale * dy[keep].astype(np.float64)))
+    if accumulate:
+        total, size = total + dtable, size + np.abs(dtable)
+    return total, size, np.bincount(ids, minlength=dtable.shape[0])
+
+
+# --------------------------------------------------------------------------------------------
+# Norm, gate and residual (norms: Prod/GPU/Kernels/SinglePrecision.cu:32-297,1345), in float64
+# --------------------------------------------------------------------------------------------
+def norm_statistics(t, kind, epsilon):
+    t = t.astype(np.float64)
+    mean = t.mean(1) if kind == "layer" else np.zeros(len(t))
+    return np.stack((mean, 1 / np.sqrt(((t - mean[:, None]) ** 2).mean(1) + epsilon)), 1)
+
+
+def norm_apply(t, stats, gamma, beta):
+    y = (t.astype(np.float64) - stats[:, :1]) * stats[:, 1:]
+    y = y if gamma is None else y * gamma
+    return y if beta is None else y + beta
+
+
+def residual_norm_sum(x, block, post_stats, p, gate_rows, residual_scale, block_scale):
+    """r of the forward pass; ``post_stats`` None: no norm behind the block; ``p``: the parameters by name."""
+    r = residual_scale * x.astype(np.float64)
+    if block is None:
+        return r
+    u = block.astype(np.float64) if post_stats is None else norm_apply(block, post_stats, p["post_gamma"], p["post_beta"])
+    if gate_rows:
+        u = u * np.repeat(p["gate"].astype(np.float64), len(x) // gate_rows, 0)
+    return r + block_scale * u
+
+
+def norm_input_gradient(g, xhat, rstd, kind):
+    centre = g.mean(1, keepdims=True) if kind == "layer" else 0.0
+    return rstd * (g - centre - xhat * (g * xhat).mean(1, keepdims=True))
+
+
+def residual_norm_backward(r, block, dy, dr, stats, post_stats, p, norm, post_norm, gate_rows, residual_scale, block_scale):
+    """Gradients by name, by the formulas of the operator from the statistics given."""
+    out = {}
+    total = np.zeros(r.shape) if dr is None else dr.astype(np.float64)
+    if norm != "none":
+        xhat, g = norm_apply(r, stats, None, None), dy.astype(np.float64)
+        out["gamma"], out["beta"] = (g * xhat).sum(0), g.sum(0)
+        g = g if p["gamma"] is None else g * p["gamma"]
+        total = total + norm_input_gradient(g, xhat, stats[:, 1:], norm)
+    out["dx"] = residual_scale * total
+    du = block_scale * total
+    if block is not None:
+        hhat = block.astype(np.float64) if post_norm == "none" else norm_apply(block, post_stats, None, None)
+        if gate_rows:
+            u = hhat
+            if post_norm != "none":
+                u = u if p["post_gamma"] is None else u * p["post_gamma"]
+                u = u if p["post_beta"] is None else u + p["post_beta"]
+            out["gate"] = (du * u).reshape(gate_rows, -1, r.shape[1]).sum(1)
+            du = du * np.repeat(p["gate"].astype(np.float64), len(r) // gate_rows, 0)
+        if post_norm != "none":
+            out["post_gamma"], out["post_beta"] = (du * hhat).sum(0), du.sum(0)
+            g = du if p["post_gamma"] is None else du * p["post_gamma"]
+            du = norm_input_gradient(g, hhat, post_stats[:, 1:], post_norm)
+    out["dblock"] = du
+    return out
+
+
+# --------------------------------------------------------------------------------------------
 # Dense layer
 # --------------------------------------------------------------------------------------------
 def dense_forward(x, W, bias, act=ACT_IDENTITY, w_layout=W_OUT_IN, f64=False, alpha=0.0):

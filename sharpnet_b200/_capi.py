@@ -20,6 +20,8 @@ ACT_LN = 1004
 ACT_CLIPPED_RELU = 3                # ceiling 1.0, as the reference's cuDNN descriptors have it
 ACT_SOFTMAX = 1000   # snb200_dense_fwd only
 W_OUT_IN, W_IN_OUT = 0, 1
+INDEX_INT32, INDEX_INT64, INDEX_FP32 = 0, 1, 2
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 LOSS_BINARY_CROSSENTROPY, LOSS_CATEGORICAL_CROSSENTROPY, LOSS_MSE = 0, 1, 2
 (TUNE_FORCE_PATH, TUNE_FORCE_BN, TUNE_REWRITE_HI, TUNE_CHUNK_K, TUNE_PAIR, TUNE_SPLITK, TUNE_VARIANT, TUNE_PDL,
  TUNE_FORCE_SPLITS, TUNE_NO_TS, TUNE_NO_FUSED_ATTN, TUNE_NO_SWLOAD, TUNE_SM_RESERVE, TUNE_CLUSTER) = range(14)
@@ -45,6 +47,20 @@ class MhaWeights(_c.Structure):     # snb200_mha_weights and snb200_mha_gradient
 
 class MhaState(_c.Structure):       # snb200_mha_state
     _fields_ = [(n, _P) for n in ("Q_heads_T", "K_heads_T", "V_heads_T", "attention_heads_T", "weights_buffer")]
+
+
+class AdamTensor(_c.Structure):     # snb200_adam_tensor
+    _fields_ = [("count", _L), ("dW", _P), ("W", _P), ("adam_vW", _P), ("adam_sW", _P), ("v_scale", _P), ("s_scale", _P),
+                ("decay", _c.c_double)]
+
+
+class NormDesc(_c.Structure):       # snb200_norm_desc
+    _fields_ = [("rows", _L)] + [(n, _I) for n in ("dim", "norm", "post_norm", "gate_rows")] + \
+               [(n, _F) for n in ("residual_scale", "block_scale", "epsilon")]
+
+
+class NormParams(_c.Structure):     # snb200_norm_params and snb200_norm_gradients (same field order)
+    _fields_ = [(n, _P) for n in ("gamma", "beta", "post_gamma", "post_beta", "gate")]
 
 
 # name -> (restype, argtypes); every symbol include/sharpnet_b200.h declares.
@@ -87,6 +103,15 @@ SIGNATURES = {
                            _c.POINTER(MhaWeights), _P, _P, _P]),
     "snb200_sgd_update": (_I, [_H, _L, _F, _F, _I, _P, _P, _P]),
     "snb200_adam_update": (_I, [_H, _L, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _I, _P, _P, _P, _P]),
+    "snb200_adam_group_update": (_I, [_H, _I, _c.POINTER(AdamTensor), _I, _c.c_double, _c.c_double, _c.c_double, _c.c_double,
+                                      _c.c_double, _I, _c.c_uint]),
+    "snb200_embedding_fwd": (_I, [_H, _I, _L, _I, _I, _P, _F, _P, _P]),
+    "snb200_embedding_scratch_bytes": (_L, [_L, _I, _I]),
+    "snb200_embedding_bwd": (_I, [_H, _I, _L, _I, _I, _P, _F, _I, _I, _P, _P, _P]),
+    "snb200_residual_norm_fwd": (_I, [_H, _c.POINTER(NormDesc), _c.POINTER(NormParams), _P, _P, _P, _P, _P, _P]),
+    "snb200_residual_norm_scratch_floats": (_L, [_c.POINTER(NormDesc)]),
+    "snb200_residual_norm_bwd": (_I, [_H, _c.POINTER(NormDesc), _c.POINTER(NormParams), _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                      _c.POINTER(NormParams)]),
     "snb200_comm_get_unique_id": (_I, [_P]),
     "snb200_comm_init_rank": (_I, [_H, _I, _I, _P]),
     "snb200_comm_init_all": (_I, [_c.POINTER(_H), _I]),

@@ -10,11 +10,14 @@
 #include <string.h>
 
 #include "../../include/sharpnet_b200.h"
+#include "adam_group.cuh"
 #include "elementwise.cuh"
+#include "embedding.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_umma.cuh"
 #include "gemm_umma2.cuh"
 #include "attention_umma.cuh"
+#include "residual_norm.cuh"
 
 using namespace snb;
 
@@ -210,6 +213,8 @@ extern "C" int snb200_check_device_status(snb200_handle_t h) {
   SNB_CUDA(h, cudaMemcpy(&w, h->error_word, sizeof(int), cudaMemcpyDeviceToHost));
   if (w) {
     cudaMemset(h->error_word, 0, sizeof(int));
+    if (w == kErrorTokenIndex)
+      return fail(h, SNB200_STATUS_INVALID_VALUE, "an embedding call was given a token index outside its table");
     return fail(h, SNB200_STATUS_EXECUTION_FAILED, "a tensor-core pipeline wait timed out on the device");
   }
   return 0;
@@ -247,7 +252,7 @@ extern "C" int snb200_selftest_wait_timeout(snb200_handle_t h, int limit_us) {
 // here starts with pdl_prologue() (or, for the tensor-core kernels, runs its set-up first), so its launch latency
 // overlaps the tail of the previous kernel and it waits for that kernel before touching memory.
 template <typename... KArgs, typename... Args>
-static void launch_pdl(snb200_handle_t h, void (*kernel)(KArgs...), dim3 grid, dim3 block, Args&&... args) {
+static void launch_pdl_smem(snb200_handle_t h, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cudaLaunchAttribute attr[1];
@@ -255,11 +260,15 @@ static void launch_pdl(snb200_handle_t h, void (*kernel)(KArgs...), dim3 grid, d
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
   cfg.blockDim = block;
-  cfg.dynamicSmemBytes = 0;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = h->stream;
   cfg.attrs = attr;
   cfg.numAttrs = h->tune[TUNE_PDL] == 1 ? 0 : 1;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);   // errors surface in check_launch (cudaGetLastError)
+}
+template <typename... KArgs, typename... Args>
+static void launch_pdl(snb200_handle_t h, void (*kernel)(KArgs...), dim3 grid, dim3 block, Args&&... args) {
+  launch_pdl_smem(h, kernel, grid, block, 0, static_cast<Args&&>(args)...);
 }
 
 // ------------------------------------------------------------------------------------ GEMM
@@ -1572,6 +1581,353 @@ extern "C" int snb200_adam_update(snb200_handle_t h, long long count, double lea
     launch_pdl(h, adam_update_kernel<1>, dim3(ew_grid(h, count, 256)), dim3(256), count, b1, b2, ep, wd, fc, dW, W, adam_vW, adam_sW);
   note_kernel(h, "adam_update", 1);
   return check_launch(h, "adam_update launch");
+}
+
+// ------------------------------------------------------------------------------------ Adam over many tensors
+struct ByteRange { const char *begin, *end; };
+static int compare_ranges(const void* a, const void* b) {
+  const char *x = static_cast<const ByteRange*>(a)->begin, *y = static_cast<const ByteRange*>(b)->begin;
+  return x < y ? -1 : x > y;
+}
+// Whether no two of the n ranges overlap; sorts them unless they come in ascending order.
+static bool disjoint(ByteRange* r, int n) {
+  for (int pass = 0; pass < 2; ++pass) {
+    int i = 1;
+    while (i < n && r[i - 1].end <= r[i].begin) ++i;
+    if (i >= n) return true;
+    if (pass == 0) qsort(r, n, sizeof(*r), compare_ranges);
+  }
+  return false;
+}
+
+template <int N>
+static int launch_adam_group(snb200_handle_t h, const snb200_adam_tensor* tensors, int* next, int n, int state_bits,
+                             const AdamCoefficients& c, double weight_decay, unsigned seed) {
+  AdamTable<N> table;
+  table.n = 0;
+  unsigned long long items = 0;
+  const int chunk = state_bits == 8 ? kAdamChunk8 : kAdamChunk32;
+  for (; *next < n && table.n < N; ++*next) {
+    const snb200_adam_tensor& s = tensors[*next];
+    if (s.count == 0) continue;
+    AdamTensor& t = table.t[table.n];
+    t.g = s.dW; t.w = s.W; t.v = s.adam_vW; t.s = s.adam_sW; t.v_scale = s.v_scale; t.s_scale = s.s_scale;
+    t.count = s.count;
+    t.weight_decay = static_cast<float>(weight_decay * s.decay);
+    const uintptr_t moments = reinterpret_cast<uintptr_t>(s.adam_vW) | reinterpret_cast<uintptr_t>(s.adam_sW);
+    const bool vec = aligned16(s.dW) && aligned16(s.W) && (moments & (state_bits == 8 ? 3u : 15u)) == 0;
+    t.ordinal_vec = static_cast<unsigned>(*next) << 1 | (vec ? 1u : 0u);
+    table.first[table.n++] = static_cast<unsigned>(items);
+    items += (static_cast<unsigned long long>(s.count) + chunk - 1) / chunk;
+    if (items > 0x7fffffffull) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "more parameters than one call updates");
+  }
+  if (table.n == 0) return 0;
+  table.total = static_cast<unsigned>(items);
+  const unsigned cap = 8u * h->sm_count;
+  const dim3 grid(table.total < cap ? table.total : cap);
+  if (state_bits == 8) launch_pdl(h, adam_group8_kernel<N>, grid, dim3(kAdamThreads), table, c, seed);
+  else launch_pdl(h, adam_group32_kernel<N>, grid, dim3(kAdamThreads), table, c);
+  note_kernel(h, state_bits == 8 ? "adam_group8" : "adam_group32", 1);
+  return check_launch(h, "adam_group launch");
+}
+
+extern "C" int snb200_adam_group_update(snb200_handle_t h, int n, const snb200_adam_tensor* tensors, int state_bits,
+                                        double learning_rate, double beta1, double beta2, double epsilon,
+                                        double weight_decay, int time_step, unsigned int rounding_seed) {
+  int st = enter(h);
+  if (st) return st;
+  if (n < 0 || time_step < 1) return fail(h, SNB200_STATUS_INVALID_VALUE, "negative number of tensors or time step below 1");
+  if (state_bits != 8 && state_bits != 32) return fail(h, SNB200_STATUS_INVALID_VALUE, "moments of %d bits: 8 or 32", state_bits);
+  if (n == 0) return 0;
+  if (!tensors) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  ByteRange* ranges = static_cast<ByteRange*>(malloc(sizeof(ByteRange) * static_cast<size_t>(n)));
+  if (!ranges) return fail(h, SNB200_STATUS_ALLOC_FAILED, "out of host memory");
+  for (int k = 0; k < 5 && !st; ++k) {      // the arrays that are written: of one kind, no two may share memory
+    if (k >= 3 && state_bits == 32) break;
+    int m = 0;
+    for (int i = 0; i < n && !st; ++i) {
+      const snb200_adam_tensor& t = tensors[i];
+      if (t.count < 0) st = fail(h, SNB200_STATUS_INVALID_VALUE, "tensor %d: negative count", i);
+      else if (t.count > 0x7fffffffffffll) st = fail(h, SNB200_STATUS_NOT_SUPPORTED, "tensor %d: %lld elements", i, t.count);
+      else if (t.count > 0) {
+        const void* p[5] = {t.W, t.adam_vW, t.adam_sW, t.v_scale, t.s_scale};
+        if (!p[k] || !t.dW) st = fail(h, SNB200_STATUS_INVALID_VALUE, "tensor %d: null pointer", i);
+        const size_t bytes = k >= 3 ? 4 * ((static_cast<size_t>(t.count) + kAdamBlock8 - 1) / kAdamBlock8)
+                                    : static_cast<size_t>(t.count) * ((k == 0 || state_bits == 32) ? 4 : 1);
+        ranges[m].begin = static_cast<const char*>(p[k]);
+        ranges[m].end = ranges[m].begin + bytes;
+        ++m;
+      }
+    }
+    if (!st && !disjoint(ranges, m)) st = fail(h, SNB200_STATUS_INVALID_VALUE, "two tensors of the list share memory");
+  }
+  free(ranges);
+  if (st) return st;
+  const double b1p = pow(beta1, time_step), b2p = pow(beta2, time_step);
+  AdamCoefficients c;
+  c.factor = static_cast<float>(learning_rate * (sqrt(1.0 - b2p) / (1.0 - b1p)));
+  c.beta1 = static_cast<float>(beta1); c.beta2 = static_cast<float>(beta2); c.eps = static_cast<float>(epsilon);
+  for (int next = 0; next < n && !st;)
+    st = n - next <= 32 ? launch_adam_group<32>(h, tensors, &next, n, state_bits, c, weight_decay, rounding_seed)
+                        : launch_adam_group<kAdamMaxTensors>(h, tensors, &next, n, state_bits, c, weight_decay, rounding_seed);
+  return st;
+}
+
+// ------------------------------------------------------------------------------------ embedding
+static int check_index_type(snb200_handle_t h, int index_type, const void* indices) {
+  if (index_type != SNB200_INDEX_INT32 && index_type != SNB200_INDEX_INT64 && index_type != SNB200_INDEX_FP32)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "unknown index type %d", index_type);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(indices);
+  if (at & (index_type == SNB200_INDEX_INT64 ? 7u : 3u)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the indices are not aligned to their type");
+  return 0;
+}
+
+extern "C" int snb200_embedding_fwd(snb200_handle_t h, int index_type, long long tokens, int vocabulary, int dim,
+                                    const void* indices, float scale, const float* table, float* y) {
+  int st = enter(h);
+  if (st) return st;
+  if (tokens < 0 || vocabulary < 1 || dim < 0)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension or empty vocabulary");
+  if ((st = check_index_type(h, index_type, indices))) return st;
+  if (tokens == 0 || dim == 0) return 0;
+  if (!indices || !table || !y) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  const bool vec = dim % 4 == 0 && aligned16(table) && aligned16(y);
+  const int row_vecs = vec ? dim / 4 : dim;
+  int bx = 1;
+  while (bx < row_vecs && bx < 256) bx <<= 1;
+  const int by = 256 / bx;
+  const unsigned columns = (row_vecs + bx - 1) / bx;
+  // rows of a thread that are in flight together: several where the batch fills the SMs all the same
+  const bool many = tokens * columns >= 64LL * h->sm_count * by;
+  const long long blocks = (tokens + by * (many ? 8 : 1) - 1) / (by * (many ? 8 : 1));
+  if (blocks > 0x7fffffffll || columns > 65535) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
+  const dim3 grid(static_cast<unsigned>(blocks), columns), block(bx, by);
+#define SNB_EMBED(V, T) launch_pdl(h, embedding_fwd_kernel<V, T>, grid, block, indices, index_type, tokens, vocabulary, row_vecs, scale, table, y, h->error_word)
+  if (vec) { if (many) SNB_EMBED(4, 8); else SNB_EMBED(4, 1); }
+  else { if (many) SNB_EMBED(1, 8); else SNB_EMBED(1, 1); }
+#undef SNB_EMBED
+  note_kernel(h, "embedding_fwd", 1);
+  return check_launch(h, "embedding_fwd launch");
+}
+
+// How the gradient of an embedding is cut, from its sizes alone (the scratch size must not depend on the device).
+struct EmbeddingPlan {
+  int tile, tiles;             // tokens of one sorting block
+  int passes, bits;            // digits of the sort and their width
+  int chunk, chunks, slabs;    // sorted tokens of one warp of the sums; slabs of columns
+  size_t keys[2], pos[2], counts, totals, partial, bytes;   // offsets in the scratch memory
+};
+static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingPlan* p) {
+  if (tokens < 0 || tokens > (1ll << 30) || vocabulary < 1 || dim < 0) return false;
+  const long long n = tokens;
+  p->tiles = static_cast<int>((n + 2047) / 2048);
+  if (p->tiles > 512) p->tiles = 512;
+  if (p->tiles < 1) p->tiles = 1;
+  p->tile = static_cast<int>((n + p->tiles - 1) / p->tiles);
+  p->tile = (p->tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+  p->tiles = static_cast<int>((n + p->tile - 1) / (p->tile ? p->tile : 1));
+  int key_bits = 0;
+  while (key_bits < 31 && (static_cast<long long>(vocabulary) >> key_bits) != 0) ++key_bits;   // keys 0 .. vocabulary
+  p->passes = (key_bits + kSortMaxBits - 1) / kSortMaxBits;
+  p->bits = (key_bits + p->passes - 1) / p->passes;
+  p->slabs = (dim + kSlab - 1) / kSlab;
+  // a warp sums `chunk` sorted tokens: as many as leave enough warps to fill the GPU
+  p->chunk = 128;
+  while (p->chunk > 8 && (n + p->chunk - 1) / p->chunk * p->slabs < 4096) p->chunk >>= 1;
+  p->chunks = static_cast<int>((n + p->chunk - 1) / p->chunk);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+  for (int k = 0; k < 2; ++k) { p->keys[k] = take(4 * static_cast<size_t>(n)); p->pos[k] = take(4 * static_cast<size_t>(n)); }
+  p->counts = take(4 * static_cast<size_t>(kSortMaxBins) * p->tiles);
+  p->totals = take(4 * kSortMaxBins);
+  p->partial = take(8 * static_cast<size_t>(p->chunks) * dim);
+  p->bytes = at;
+  return true;
+}
+extern "C" long long snb200_embedding_scratch_bytes(long long tokens, int vocabulary, int dim) {
+  EmbeddingPlan p;
+  return embedding_plan(tokens, vocabulary, dim, &p) ? static_cast<long long>(p.bytes) : -1;
+}
+
+extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long tokens, int vocabulary, int dim,
+                                    const void* indices, float scale, int padding_index, int accumulate, const float* dy,
+                                    void* scratch, float* dtable) {
+  int st = enter(h);
+  if (st) return st;
+  if (tokens < 0 || vocabulary < 1 || dim < 0)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension or empty vocabulary");
+  if ((st = check_index_type(h, index_type, indices))) return st;
+  EmbeddingPlan plan;
+  if (!embedding_plan(tokens, vocabulary, dim, &plan)) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "more than 2^30 tokens");
+  if (dim == 0 || (tokens == 0 && accumulate)) return 0;
+  if (!dtable || (tokens > 0 && (!indices || !dy || !scratch))) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  if (!aligned16(scratch)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the scratch memory is not aligned to 16 bytes");
+  int launches = 0;
+  if (!accumulate) {
+    const long long count = static_cast<long long>(vocabulary) * dim;
+    launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, count / 4 + 1, 256)), dim3(256), count, dtable);
+    ++launches;
+  }
+  if (tokens > 0) {
+    char* base = static_cast<char*>(scratch);
+    SortPass s;
+    memset(&s, 0, sizeof(s));
+    s.indices = indices; s.index_type = index_type; s.vocab = vocabulary; s.padding = padding_index;
+    s.counts = reinterpret_cast<unsigned*>(base + plan.counts);
+    s.totals = reinterpret_cast<unsigned*>(base + plan.totals);
+    s.n = static_cast<int>(tokens); s.tile = plan.tile; s.tiles = plan.tiles;
+    s.bits = plan.bits; s.error_word = h->error_word;
+    for (int pass = 0; pass < plan.passes; ++pass) {
+      s.first = pass == 0; s.shift = pass * plan.bits;
+      s.keys_in = reinterpret_cast<unsigned*>(base + plan.keys[(pass + 1) & 1]);
+      s.pos_in = reinterpret_cast<unsigned*>(base + plan.pos[(pass + 1) & 1]);
+      s.keys_out = reinterpret_cast<unsigned*>(base + plan.keys[pass & 1]);
+      s.pos_out = reinterpret_cast<unsigned*>(base + plan.pos[pass & 1]);
+      launch_pdl(h, sort_count_kernel, dim3(plan.tiles), dim3(kSortThreads), s);
+      launch_pdl(h, sort_prefix_kernel, dim3(((1u << plan.bits) + 7) / 8), dim3(256), s);
+      launch_pdl_smem(h, sort_scatter_kernel, dim3(plan.tiles), dim3(kSortThreads), (static_cast<size_t>(4) << plan.bits) * kSortWarps, s);
+      launches += 3;
+    }
+    WordSums w;
+    memset(&w, 0, sizeof(w));
+    w.keys = s.keys_out; w.pos = s.pos_out;
+    w.n = s.n; w.vocab = vocabulary; w.dim = dim; w.chunk = plan.chunk; w.chunks = plan.chunks; w.slabs = plan.slabs;
+    w.scale = scale; w.accumulate = accumulate ? 1 : 0; w.dy = dy; w.dtable = dtable;
+    w.partial = reinterpret_cast<float*>(base + plan.partial);
+    const long long blocks = (static_cast<long long>(plan.chunks) * plan.slabs + 7) / 8;
+    if (blocks > 0x7fffffffll) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
+    const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (vec) { launch_pdl(h, word_sums_kernel<4>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<4>, grid, dim3(256), w); }
+    else { launch_pdl(h, word_sums_kernel<1>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<1>, grid, dim3(256), w); }
+    launches += 2;
+  }
+  note_kernel(h, "embedding_bwd", launches);
+  return check_launch(h, "embedding_bwd launch");
+}
+
+// ------------------------------------------------------------------------------------ norm, gate and residual
+static int norm_check(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p) {
+  if (!d || !p) return fail(h, SNB200_STATUS_INVALID_VALUE, "null descriptor or parameters");
+  if (d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension");
+  const int kinds[2] = {d->norm, d->post_norm};
+  for (int k = 0; k < 2; ++k)
+    if (kinds[k] != SNB200_NORM_NONE && kinds[k] != SNB200_NORM_LAYER && kinds[k] != SNB200_NORM_RMS)
+      return fail(h, SNB200_STATUS_INVALID_VALUE, "unknown norm %d", kinds[k]);
+  if (!(d->epsilon > 0.0f)) return fail(h, SNB200_STATUS_INVALID_VALUE, "epsilon must be above zero");
+  if (d->gate_rows > 0 && (d->gate_rows > d->rows || d->rows % d->gate_rows != 0) && d->rows > 0)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "%lld rows cannot share %d rows of the gate equally", d->rows, d->gate_rows);
+  if ((d->gate_rows > 0) != (p->gate != nullptr)) return fail(h, SNB200_STATUS_INVALID_VALUE, "gate_rows and gate do not agree");
+  if (d->norm == SNB200_NORM_NONE && (p->gamma || p->beta)) return fail(h, SNB200_STATUS_INVALID_VALUE, "gamma or beta without a norm");
+  if (d->post_norm == SNB200_NORM_NONE && (p->post_gamma || p->post_beta))
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "post_gamma or post_beta without a norm behind the block");
+  return 0;
+}
+
+extern "C" int snb200_residual_norm_fwd(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p, const float* x,
+                                        const float* block, float* r, float* y, float* stats, float* post_stats) {
+  int st = enter(h);
+  if (st) return st;
+  if ((st = norm_check(h, d, p))) return st;
+  if (d->rows == 0 || d->dim == 0) return 0;
+  if (!x || (d->norm != SNB200_NORM_NONE && !y)) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  if (!block && (d->post_norm != SNB200_NORM_NONE || p->gate))
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "a gate or a norm behind the block without a block");
+  if (!r && (block || d->norm == SNB200_NORM_NONE)) return fail(h, SNB200_STATUS_INVALID_VALUE, "no room for the residual sum");
+  NormArgs a;
+  memset(&a, 0, sizeof(a));
+  a.rows = d->rows; a.dim = d->dim; a.norm = d->norm; a.post = d->post_norm; a.gate_rows = d->gate_rows;
+  a.rows_per_gate = d->gate_rows > 0 ? d->rows / d->gate_rows : d->rows;
+  a.a = d->residual_scale; a.b = d->block_scale; a.eps = d->epsilon;
+  a.gamma = p->gamma; a.beta = p->beta; a.post_gamma = p->post_gamma; a.post_beta = p->post_beta; a.gate = p->gate;
+  a.x = x; a.h = block; a.r = r; a.y = y; a.stats = stats; a.post_stats = post_stats;
+  const long long cap = 16LL * h->sm_count;
+  launch_pdl(h, residual_norm_fwd_wide_kernel, dim3(static_cast<unsigned>(d->rows < cap ? d->rows : cap)), dim3(256), a);
+  note_kernel(h, "residual_norm_fwd", 1);
+  return check_launch(h, "residual_norm_fwd launch");
+}
+
+// How the rows of the backward pass are dealt out, from the sizes alone (the scratch size must not depend on the
+// device): units of consecutive rows that share a row of the gate, and the teams that take them in turn.
+constexpr int kNormTeams = 296;
+struct NormPlan { int pieces, units, teams; };
+static NormPlan norm_plan(const snb200_norm_desc* d) {
+  NormPlan n;
+  const long long groups = d->gate_rows > 1 ? d->gate_rows : 1, per = d->rows / groups;
+  long long pieces = groups == 1 ? kNormTeams : (2 * kNormTeams + groups - 1) / groups;
+  if (pieces > per) pieces = per;
+  if (pieces < 1) pieces = 1;
+  n.pieces = static_cast<int>(pieces);
+  n.units = static_cast<int>(groups * pieces);
+  n.teams = n.units < kNormTeams ? n.units : kNormTeams;
+  return n;
+}
+extern "C" long long snb200_residual_norm_scratch_floats(const snb200_norm_desc* d) {
+  if (!d || d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return -1;
+  const NormPlan n = norm_plan(d);
+  const long long sums = 2 * (d->norm != SNB200_NORM_NONE) + 2 * (d->post_norm != SNB200_NORM_NONE);
+  return (sums * n.teams + (d->gate_rows > 0 && n.pieces > 1 ? n.units : 0)) * d->dim;
+}
+
+extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p, const float* r,
+                                        const float* block, const float* dy, const float* dr, const float* stats,
+                                        const float* post_stats, float* scratch, float* dx, float* dblock,
+                                        const snb200_norm_gradients* gradients) {
+  int st = enter(h);
+  if (st) return st;
+  if ((st = norm_check(h, d, p))) return st;
+  snb200_norm_gradients none;
+  memset(&none, 0, sizeof(none));
+  const snb200_norm_gradients g = gradients ? *gradients : none;
+  if ((g.gamma && !p->gamma) || (g.beta && !p->beta) || (g.post_gamma && !p->post_gamma) || (g.post_beta && !p->post_beta) ||
+      (g.gate && !p->gate))
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "a gradient of a parameter that is not there");
+  if (!dx && !dblock && !g.gamma && !g.beta && !g.post_gamma && !g.post_beta && !g.gate)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "no output is wanted");
+  if (d->dim == 0) return 0;
+  float* vectors[SUM_COUNT] = {g.gamma, g.beta, g.post_gamma, g.post_beta};
+  if (d->rows == 0) {                       // no rows: the sums are zero
+    for (int k = 0; k < SUM_COUNT; ++k)
+      if (vectors[k]) launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, d->dim, 256)), dim3(256), d->dim, vectors[k]);
+    if (g.gate) launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, d->dim, 256)), dim3(256), static_cast<long long>(d->gate_rows) * d->dim, g.gate);
+    return check_launch(h, "residual_norm_bwd launch");
+  }
+  if (d->norm != SNB200_NORM_NONE && (!r || !dy || !stats)) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  if (d->norm == SNB200_NORM_NONE && !dr) return fail(h, SNB200_STATUS_INVALID_VALUE, "no gradient comes in");
+  if (d->post_norm != SNB200_NORM_NONE && (!block || !post_stats)) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
+  if (g.gate && !block) return fail(h, SNB200_STATUS_INVALID_VALUE, "the gradient of the gate needs the block");
+  const NormPlan plan = norm_plan(d);
+  NormGradArgs a;
+  memset(&a, 0, sizeof(a));
+  a.rows = d->rows; a.dim = d->dim; a.norm = d->norm; a.post = d->post_norm; a.gate_rows = d->gate_rows;
+  a.rows_per_gate = d->gate_rows > 0 ? d->rows / d->gate_rows : d->rows;
+  a.a = d->residual_scale; a.b = d->block_scale;
+  a.gamma = p->gamma; a.post_gamma = p->post_gamma; a.post_beta = p->post_beta; a.gate = p->gate;
+  a.r = r; a.h = (g.gate || d->post_norm != SNB200_NORM_NONE) ? block : nullptr;
+  a.dy = dy; a.dr = dr; a.stats = stats; a.post_stats = post_stats; a.dx = dx; a.dh = dblock;
+  a.pieces = plan.pieces; a.units = plan.units;
+  for (int k = 0; k < SUM_COUNT; ++k) a.slot[k] = vectors[k] ? a.sums++ : -1;
+  const bool split_gate = g.gate && plan.pieces > 1;
+  if ((a.sums > 0 || split_gate) && !scratch) return fail(h, SNB200_STATUS_INVALID_VALUE, "no scratch memory");
+  if (!aligned16(scratch)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the scratch memory is not aligned to 16 bytes");
+  a.partial = scratch;
+  a.dgate = g.gate;
+  a.gate_partial = scratch + static_cast<long long>(plan.teams) * a.sums * d->dim;
+  int launches = 1;
+  launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.teams), dim3(256), a);
+  const unsigned columns = (d->dim + 31) / 32;
+  for (int k = 0; k < SUM_COUNT; ++k) {
+    if (!vectors[k]) continue;
+    launch_pdl(h, norm_sums_kernel, dim3(columns, 1), dim3(256), a.partial + static_cast<long long>(a.slot[k]) * d->dim,
+               static_cast<long long>(a.sums) * d->dim, plan.teams, d->dim, vectors[k]);
+    ++launches;
+  }
+  if (split_gate) {
+    launch_pdl(h, norm_sums_kernel, dim3(columns, d->gate_rows), dim3(256), a.gate_partial, static_cast<long long>(d->dim), plan.pieces, d->dim, g.gate);
+    ++launches;
+  }
+  note_kernel(h, "residual_norm_bwd", launches);
+  return check_launch(h, "residual_norm_bwd launch");
 }
 
 // ------------------------------------------------------------------------------------ attention
