@@ -1841,32 +1841,62 @@ extern "C" int snb200_residual_norm_fwd(snb200_handle_t h, const snb200_norm_des
   a.a = d->residual_scale; a.b = d->block_scale; a.eps = d->epsilon;
   a.gamma = p->gamma; a.beta = p->beta; a.post_gamma = p->post_gamma; a.post_beta = p->post_beta; a.gate = p->gate;
   a.x = x; a.h = block; a.r = r; a.y = y; a.stats = stats; a.post_stats = post_stats;
+  const bool vec = d->dim % 4 == 0 && aligned16(x) && aligned16(block) && aligned16(r) && aligned16(y) && aligned16(p->gamma) &&
+                   aligned16(p->beta) && aligned16(p->post_gamma) && aligned16(p->post_beta) && aligned16(p->gate);
   const long long cap = 16LL * h->sm_count;
-  launch_pdl(h, residual_norm_fwd_wide_kernel, dim3(static_cast<unsigned>(d->rows < cap ? d->rows : cap)), dim3(256), a);
+#define SNB_NORM(W, V)                                                                                                    \
+  do {                                                                                                                    \
+    const long long blocks = (d->rows + (W == 1 ? 7 : 0)) / (W == 1 ? 8 : 1);                                             \
+    const dim3 grid(static_cast<unsigned>(blocks < cap ? blocks : cap)), threads(W == 1 ? 256 : 32 * W);                  \
+    if (vec) launch_pdl(h, residual_norm_fwd_kernel<W, V, 4>, grid, threads, a);                                          \
+    else launch_pdl(h, residual_norm_fwd_kernel<W, V, 1>, grid, threads, a);                                              \
+  } while (0)
+  if (d->dim <= 128) SNB_NORM(1, 1);
+  else if (d->dim <= 256) SNB_NORM(1, 2);
+  else if (d->dim <= 512) SNB_NORM(1, 4);
+  else if (d->dim <= 1024) SNB_NORM(4, 2);
+  else if (d->dim <= 2048) SNB_NORM(4, 4);
+  else if (d->dim <= 4096) SNB_NORM(8, 4);
+  else if (d->dim <= 8192) SNB_NORM(16, 4);
+  else if (d->dim <= 16384) SNB_NORM(32, 4);
+  else launch_pdl(h, residual_norm_fwd_wide_kernel, dim3(static_cast<unsigned>(d->rows < cap ? d->rows : cap)), dim3(256), a);
+#undef SNB_NORM
   note_kernel(h, "residual_norm_fwd", 1);
   return check_launch(h, "residual_norm_fwd launch");
 }
 
 // How the rows of the backward pass are dealt out, from the sizes alone (the scratch size must not depend on the
-// device): units of consecutive rows that share a row of the gate, and the teams that take them in turn.
-constexpr int kNormTeams = 296;
-struct NormPlan { int pieces, units, teams; };
+// device): units of consecutive rows that share a row of the gate, and the blocks whose teams take them in turn.
+constexpr int kNormBlocks = 296;
+struct NormPlan { int teams, pieces, units, blocks; };   // teams: of one block
 static NormPlan norm_plan(const snb200_norm_desc* d) {
   NormPlan n;
+  n.teams = d->dim <= 512 ? 8 : 1;
   const long long groups = d->gate_rows > 1 ? d->gate_rows : 1, per = d->rows / groups;
-  long long pieces = groups == 1 ? kNormTeams : (2 * kNormTeams + groups - 1) / groups;
+  const long long all = static_cast<long long>(kNormBlocks) * n.teams;
+  long long pieces = groups == 1 ? all : (2 * all + groups - 1) / groups;
   if (pieces > per) pieces = per;
   if (pieces < 1) pieces = 1;
   n.pieces = static_cast<int>(pieces);
   n.units = static_cast<int>(groups * pieces);
-  n.teams = n.units < kNormTeams ? n.units : kNormTeams;
+  n.blocks = n.units < all ? (n.units + n.teams - 1) / n.teams : kNormBlocks;
   return n;
 }
 extern "C" long long snb200_residual_norm_scratch_floats(const snb200_norm_desc* d) {
   if (!d || d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return -1;
   const NormPlan n = norm_plan(d);
   const long long sums = 2 * (d->norm != SNB200_NORM_NONE) + 2 * (d->post_norm != SNB200_NORM_NONE);
-  return (sums * n.teams + (d->gate_rows > 0 && n.pieces > 1 ? n.units : 0)) * d->dim;
+  return (sums * n.blocks + (d->gate_rows > 0 && n.pieces > 1 ? n.units : 0)) * d->dim;
+}
+
+template <int WARPS, int VPT>
+static int launch_norm_bwd(snb200_handle_t h, const NormGradArgs& a, int blocks, bool vec) {
+  const size_t smem = static_cast<size_t>(WARPS == 1 ? 8 : 1) * (a.sums + (a.dgate ? 1 : 0)) * VPT * 32 * WARPS * sizeof(float4);
+  const auto kernel = vec ? residual_norm_bwd_kernel<WARPS, VPT, 4> : residual_norm_bwd_kernel<WARPS, VPT, 1>;
+  if (smem > 40 * 1024)   // the static part counts towards the default limit of 48 KB
+    SNB_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  launch_pdl_smem(h, kernel, dim3(blocks), dim3(WARPS == 1 ? 256 : 32 * WARPS), smem, a);
+  return 0;
 }
 
 extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p, const float* r,
@@ -1912,18 +1942,28 @@ extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_des
   if (!aligned16(scratch)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the scratch memory is not aligned to 16 bytes");
   a.partial = scratch;
   a.dgate = g.gate;
-  a.gate_partial = scratch + static_cast<long long>(plan.teams) * a.sums * d->dim;
+  a.gate_partial = scratch + static_cast<long long>(plan.blocks) * a.sums * d->dim;
+  const bool vec = d->dim % 4 == 0 && aligned16(r) && aligned16(block) && aligned16(dy) && aligned16(dr) && aligned16(dx) &&
+                   aligned16(dblock) && aligned16(p->gamma) && aligned16(p->post_gamma) && aligned16(p->post_beta) &&
+                   aligned16(p->gate) && (!g.gate || aligned16(g.gate));
+  if (d->dim <= 128) st = launch_norm_bwd<1, 1>(h, a, plan.blocks, vec);
+  else if (d->dim <= 256) st = launch_norm_bwd<1, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 512) st = launch_norm_bwd<1, 4>(h, a, plan.blocks, vec);
+  else if (d->dim <= 1024) st = launch_norm_bwd<4, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 2048) st = launch_norm_bwd<4, 4>(h, a, plan.blocks, vec);
+  else if (d->dim <= 4096) st = launch_norm_bwd<8, 4>(h, a, plan.blocks, vec);
+  else if (d->dim <= 8192) st = launch_norm_bwd<16, 4>(h, a, plan.blocks, vec);
+  else launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.blocks), dim3(256), a);
+  if (st) return st;
   int launches = 1;
-  launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.teams), dim3(256), a);
-  const unsigned columns = (d->dim + 31) / 32;
-  for (int k = 0; k < SUM_COUNT; ++k) {
-    if (!vectors[k]) continue;
-    launch_pdl(h, norm_sums_kernel, dim3(columns, 1), dim3(256), a.partial + static_cast<long long>(a.slot[k]) * d->dim,
-               static_cast<long long>(a.sums) * d->dim, plan.teams, d->dim, vectors[k]);
-    ++launches;
-  }
-  if (split_gate) {
-    launch_pdl(h, norm_sums_kernel, dim3(columns, d->gate_rows), dim3(256), a.gate_partial, static_cast<long long>(d->dim), plan.pieces, d->dim, g.gate);
+  if (a.sums > 0 || split_gate) {
+    NormSums s;
+    memset(&s, 0, sizeof(s));
+    s.partial = a.partial; s.gate_partial = a.gate_partial; s.parts = plan.blocks; s.pieces = plan.pieces;
+    s.sums = a.sums; s.dim = d->dim; s.gate = g.gate;
+    for (int k = 0; k < SUM_COUNT; ++k)
+      if (vectors[k]) s.out[a.slot[k]] = vectors[k];
+    launch_pdl(h, norm_sums_kernel, dim3((d->dim + 31) / 32, a.sums + (split_gate ? d->gate_rows : 0)), dim3(1024), s);
     ++launches;
   }
   note_kernel(h, "residual_norm_bwd", launches);
