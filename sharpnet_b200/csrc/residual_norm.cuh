@@ -10,12 +10,14 @@
 //   dgamma = sum dy xhat, dbeta = sum dy, dpost_gamma = sum du hhat, dpost_beta = sum du, over the rows.
 #pragma once
 #include "elementwise.cuh"
+#include "ptx.cuh"
 
 namespace snb {
 
 enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 // column sums of the backward pass over all rows, in the order in which the scratch memory holds them
-enum NormSum : int { SUM_GAMMA = 0, SUM_BETA = 1, SUM_POST_GAMMA = 2, SUM_POST_BETA = 3, SUM_COUNT = 4 };
+// (the gate's is one of them where one gate serves all rows)
+enum NormSum : int { SUM_GAMMA = 0, SUM_BETA = 1, SUM_POST_GAMMA = 2, SUM_POST_BETA = 3, SUM_GATE = 4, SUM_COUNT = 5 };
 
 struct NormArgs {
   long long rows;
@@ -38,8 +40,9 @@ struct NormGradArgs {
   int slot[SUM_COUNT], sums;     // slot[k] is the place of NormSum k among the `sums` vectors that are wanted, or -1
   int pieces, units;             // pieces that the rows of one gate row are cut into; work units: all pieces
   float* partial;                // [teams][sums][dim]
-  float* dgate;                  // NULL where it is not wanted
+  float* dgate;                  // of a gate that changes with the rows; NULL where it is not wanted
   float* gate_partial;           // [units][dim]: the gate's sums where pieces > 1
+  int* error_word;
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -185,6 +188,8 @@ residual_norm_bwd_wide_kernel(const NormGradArgs p) {
           const float hhat = p.post != NORM_NONE ? (hv - pm) * pr : hv;
           if (p.slot[SUM_POST_GAMMA] >= 0) sums[static_cast<long long>(p.slot[SUM_POST_GAMMA]) * p.dim + c] += du * hhat;
           if (p.slot[SUM_POST_BETA] >= 0) sums[static_cast<long long>(p.slot[SUM_POST_BETA]) * p.dim + c] += du;
+          if (p.slot[SUM_GATE] >= 0)
+            sums[static_cast<long long>(p.slot[SUM_GATE]) * p.dim + c] += p.b * d * (p.post != NORM_NONE ? affine(hhat, p.post_gamma, p.post_beta, c) : hv);
           if (gate_sum) gate_sum[c] += p.b * d * (p.post != NORM_NONE ? affine(hhat, p.post_gamma, p.post_beta, c) : hv);
           if (p.dh) {
             const float g = p.post_gamma ? du * __ldg(p.post_gamma + c) : du;
@@ -336,31 +341,379 @@ residual_norm_fwd_kernel(const NormArgs p) {
   }
 }
 
-// The backward pass.  The column sums are added up in shared memory, where each thread keeps its own columns (five
-// vectors of a wide row do not fit beside the row in registers, and a second pass over the batch for them would double
-// the traffic); a block writes its sums once, when its rows are done.
+// The backward pass of rows of up to 4096 elements: blocks of 16 warps, one a SM, cut into teams of WARPS warps with a row
+// each.  A warp owns VPT * 128 consecutive columns.  It has its part of the row's r, dy, dr and h (and of the gate where
+// its rows change) copied into shared memory by bulk copies of its own, two rows ahead, on barriers of its own, so that
+// the memory pipe is busy while rows go through their two reductions and no warp waits for another's data; the thread's
+// share of the five column sums stays in registers.  What all rows read (gamma, post_gamma, post_beta, a gate for all)
+// lies in shared memory.
+// Bulk copies begin and end on 16-byte borders: a part that does not (VEC = 1) is fetched with the few bytes around it,
+// which lie in the same 16-byte granules.
+constexpr int kNormThreads = 512;
+constexpr int kNormWarps = kNormThreads / 32;
+constexpr int kNormStages = 2;
+template <int VPT> __host__ __device__ constexpr int norm_part() { return VPT * 512 + 16; }       // bytes of a warp's part of a row, as fetched
+
+__device__ __forceinline__ void bulk_copy(void* smem, const void* global, unsigned bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(smem)), "l"(global), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+
+// The rows that a team takes, in order.
+struct NormRows {
+  int unit;
+  long long row, end;
+  __device__ __forceinline__ void start(const NormGradArgs& p, int first) {
+    unit = first;
+    if (unit < p.units) norm_unit_rows(p, unit, &row, &end);
+  }
+  __device__ __forceinline__ void next(const NormGradArgs& p, int stride) {
+    if (++row < end) return;
+    unit += stride;
+    if (unit < p.units) norm_unit_rows(p, unit, &row, &end);
+  }
+};
+
+// Two sums over a team of WARPS warps, in a fixed order.  The lower half of a warp adds up x and the upper half y, which
+// takes one exchange instead of a second chain of five; barrier 1 + team is the team's own, `red` is used in turn by
+// `flip` so that one barrier a sum is enough.
+template <int WARPS>
+__device__ __forceinline__ float2 team_sum_pair(float2 v, float (*red)[2][kNormWarps], int team, int& flip) {
+  const int lane = threadIdx.x & 31, half = lane >> 4;
+  float s = half ? v.y : v.x;
+  s += __shfl_xor_sync(0xffffffffu, half ? v.x : v.y, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (WARPS > 1) {
+    const int warp = threadIdx.x >> 5;
+    if ((lane & 15) == 0) red[flip][half][warp] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * WARPS) : "memory");
+    s = (lane & 15) < WARPS ? red[flip][half][team * WARPS + (lane & 15)] : 0.0f;
+    flip ^= 1;
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+  return make_float2(__shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, s, 16));
+}
+
+// Two floats a register pair: sm_100a adds, multiplies and fuses both in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Elements of group j of a warp's part, in pairs: one 16-byte vector a lane (VEC = 4), or four elements 32 apart (VEC = 1);
+// zeros behind the row's end (`left`: columns from the lane's first to the row's end).
+struct Pairs { float2 a, b; };
+template <int VEC>
+__device__ __forceinline__ Pairs part_load(const float* part, int j, int lane, int left) {
+  if (VEC == 4) {
+    const float4 v = 128 * j < left ? *reinterpret_cast<const float4*>(part + 128 * j + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return Pairs{make_float2(v.x, v.y), make_float2(v.z, v.w)};
+  }
+  const float* e = part + 128 * j + lane;
+  float v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = 128 * j + 32 * k < left ? e[32 * k] : 0.0f;
+  return Pairs{make_float2(v[0], v[1]), make_float2(v[2], v[3])};
+}
+// The same of a parameter vector in global memory; `fill` where there is none.
+template <int VEC>
+__device__ __forceinline__ Pairs param_pairs(const float* v, int mine, int j, int left, float fill) {
+  float e[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = 128 * j + (VEC == 4 ? k : 32 * k);
+    e[k] = !v ? fill : c < left ? __ldg(v + mine + c) : 0.0f;
+  }
+  return Pairs{make_float2(e[0], e[1]), make_float2(e[2], e[3])};
+}
+// `row`: at the lane's first column.
+template <int VEC>
+__device__ __forceinline__ void part_store(float* row, int j, int left, const Pairs& v) {
+  if (VEC == 4) {
+    if (128 * j < left) __stcs(reinterpret_cast<float4*>(row + 128 * j), make_float4(v.a.x, v.a.y, v.b.x, v.b.y));
+    return;
+  }
+  const float e[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (128 * j + 32 * k < left) __stcs(row + 128 * j + 32 * k, e[k]);
+}
+
+// Per row, with e = b dR:  A += e hhat and B += e.  A gate's gradient is post_gamma A + post_beta B over its rows, those of
+// post_gamma and post_beta are gate A and gate B summed over the gates, so the loop over rows needs neither parameter by
+// itself: only b gate post_gamma, which is one vector unless the gate changes with the rows (GATES: it does; its rows come
+// as a fifth stream).
+template <int WARPS, int VPT, int VEC, bool GATES>
+static __global__ void __launch_bounds__(kNormThreads, 1)
+residual_norm_bwd_kernel(const NormGradArgs p) {
+  pdl_prologue();
+  constexpr int TEAMS = kNormWarps / WARPS, COLUMNS = WARPS * VPT * 128, PART = norm_part<VPT>();
+  extern __shared__ float4 norm_smem[];   // [warps][stages][streams][PART bytes], [2][COLUMNS]
+  __shared__ float red[2][2][kNormWarps];
+  __shared__ float stat_slots[kNormWarps][kNormStages][4];
+  __shared__ uint64_t bars[kNormWarps][kNormStages];
+  __shared__ int abort_flag;
+  int flip = 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / WARPS, stride = gridDim.x * TEAMS;
+  const int first = (warp % WARPS) * VPT * 128;                        // the warp's first column
+  const int columns = min(VPT * 128, p.dim - first);                   // and how many of its columns there are (<= 0: none)
+  const int mine = first + (VEC == 4 ? 4 * lane : lane), left = p.dim - mine;
+  const float inv_dim = 1.0f / p.dim;
+  const bool norm = p.norm != NORM_NONE, post = p.post != NORM_NONE;
+  const int at_dr = norm ? 2 : 0, at_h = at_dr + (p.dr != nullptr), at_gate = at_h + (p.h != nullptr);
+  const int streams = at_gate + GATES;
+  char* const parts = reinterpret_cast<char*>(norm_smem) + warp * kNormStages * streams * PART;
+  float* const gamma = reinterpret_cast<float*>(reinterpret_cast<char*>(norm_smem) + kNormWarps * kNormStages * streams * PART);
+  float* const back = gamma + COLUMNS;                                 // b gate post_gamma, or b post_gamma where the gates change
+  for (int i = threadIdx.x; i < COLUMNS; i += kNormThreads) {
+    const bool in = i < p.dim;
+    gamma[i] = !in ? 0.0f : p.gamma ? __ldg(p.gamma + i) : 1.0f;
+    const float g = !in ? 0.0f : !GATES && p.gate_rows ? p.b * __ldg(p.gate + i) : p.b;
+    back[i] = in && p.post_gamma ? g * __ldg(p.post_gamma + i) : g;
+  }
+  if (threadIdx.x < kNormWarps * kNormStages) mbar_init(&bars[0][0] + threadIdx.x, 1);
+  if (threadIdx.x == 0) { abort_flag = 0; fence_mbar_init(); }
+  __syncthreads();
+
+  // lane k < streams has the warp's part of stream k copied
+  const float* source = nullptr;
+  if (norm && lane < 2) source = lane == 0 ? p.r : p.dy;
+  if (p.dr && lane == at_dr) source = p.dr;
+  if (p.h && lane == at_h) source = p.h;
+  if (GATES && lane == at_gate) source = p.gate;
+  const float* const stat_source = lane < 2 ? p.stats : p.post_stats;
+  auto fetch = [&](const NormRows& it, int stage) {
+    if (it.unit < p.units) {
+      uint64_t* const bar = &bars[warp][stage];
+      const float* from = source + (GATES && lane == at_gate ? static_cast<long long>(it.unit / p.pieces) : it.row) * p.dim + first;
+      unsigned over = 0, bytes = 4 * columns;
+      if (VEC == 1) {
+        over = static_cast<unsigned>(reinterpret_cast<uintptr_t>(from) & 15);
+        bytes = (over + bytes + 15) & ~15u;
+      }
+      if (columns > 0) {
+        if (VEC == 4) {
+          if (lane == 0) mbar_arrive_expect_tx(bar, streams * bytes);
+        } else {
+          const unsigned total = __reduce_add_sync(0xffffffffu, lane < streams ? bytes : 0);
+          if (lane == 0) mbar_arrive_expect_tx(bar, total);
+        }
+        __syncwarp();
+        if (lane < streams) bulk_copy(parts + (stage * streams + lane) * PART, reinterpret_cast<const char*>(from) - over, bytes, bar);
+      } else if (lane == 0) {
+        mbar_arrive(bar);
+      }
+      if (lane < 4 && (lane < 2 ? norm : post)) copy_async4(&stat_slots[warp][stage][lane], stat_source + 2 * it.row + (lane & 1));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");       // a group a row, an empty one behind the last
+  };
+  // the warp's part of stream k, past the bytes in front of it
+  auto part_of = [&](int stage, int k, const float* row) {
+    const float* part = reinterpret_cast<const float*>(parts + (stage * streams + k) * PART);
+    return VEC == 4 ? part : part + ((reinterpret_cast<uintptr_t>(row + first) & 15) >> 2);
+  };
+  const Pairs zero = {both(0.0f), both(0.0f)};
+  Pairs sum_gamma[VPT], sum_beta[VPT], A[VPT], B[VPT], sum_post_gamma[GATES ? VPT : 1], sum_post_beta[GATES ? VPT : 1];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    sum_gamma[j] = sum_beta[j] = A[j] = B[j] = zero;
+    if (GATES) sum_post_gamma[j] = sum_post_beta[j] = zero;
+  }
+
+  NormRows now, ahead;
+  now.start(p, blockIdx.x * TEAMS + team);
+  ahead.start(p, now.unit);
+  for (int s = 0; s < kNormStages; ++s) {
+    fetch(ahead, s);
+    if (ahead.unit < p.units) ahead.next(p, stride);
+  }
+  int stage = 0;
+  unsigned parity = 0;
+  while (now.unit < p.units) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 1) : "memory");
+    __syncwarp();
+    mbar_wait(&bars[warp][stage], parity, &abort_flag);
+    const long long out = now.row * p.dim;
+    const float* const st = stat_slots[warp][stage];
+    Pairs d[VPT], x[VPT], g[VPT];
+    const float* const part_d = part_of(stage, at_dr, p.dr + out);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) d[j] = p.dr ? part_load<VEC>(part_d, j, lane, left) : zero;
+    if (norm) {
+      const float2 m = both(-st[0]), rstd = both(st[1]);
+      const float* const part_r = part_of(stage, 0, p.r + out);
+      const float* const part_g = part_of(stage, 1, p.dy + out);
+      float2 s = both(0.0f), q = both(0.0f);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const Pairs r = part_load<VEC>(part_r, j, lane, left), v = part_load<VEC>(part_g, j, lane, left);
+        const Pairs ga = part_load<VEC>(gamma + first, j, lane, 1 << 20);
+        x[j].a = mul2(add2(r.a, m), rstd); x[j].b = mul2(add2(r.b, m), rstd);
+        sum_gamma[j].a = fma2(v.a, x[j].a, sum_gamma[j].a); sum_gamma[j].b = fma2(v.b, x[j].b, sum_gamma[j].b);
+        sum_beta[j].a = add2(sum_beta[j].a, v.a); sum_beta[j].b = add2(sum_beta[j].b, v.b);
+        g[j].a = mul2(v.a, ga.a); g[j].b = mul2(v.b, ga.b);
+        s = add2(s, add2(g[j].a, g[j].b));
+        q = fma2(g[j].a, x[j].a, q); q = fma2(g[j].b, x[j].b, q);
+      }
+      const float2 c = team_sum_pair<WARPS>(make_float2(s.x + s.y, q.x + q.y), red, team, flip);
+      const float2 c1 = both(p.norm == NORM_LAYER ? -c.x * inv_dim : 0.0f), c2 = both(-c.y * inv_dim);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        d[j].a = fma2(rstd, add2(fma2(x[j].a, c2, g[j].a), c1), d[j].a);
+        d[j].b = fma2(rstd, add2(fma2(x[j].b, c2, g[j].b), c1), d[j].b);
+      }
+    }
+    if (p.dx) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) part_store<VEC>(p.dx + out + mine, j, left, Pairs{mul2(both(p.a), d[j].a), mul2(both(p.a), d[j].b)});
+    }
+    float2 s = both(0.0f), q = both(0.0f);
+    float2 pr = both(1.0f);
+    if (p.h || p.dh) {
+      const float2 pm = both(post ? -st[2] : 0.0f);
+      if (post) pr = both(st[3]);
+      const float* const part_h = part_of(stage, at_h, p.h + out);
+      const float* const part_gate = part_of(stage, at_gate, GATES ? p.gate + static_cast<long long>(now.unit / p.pieces) * p.dim : nullptr);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const Pairs h = p.h ? part_load<VEC>(part_h, j, lane, left) : zero;
+        Pairs bk = part_load<VEC>(back + first, j, lane, 1 << 20);
+        if (GATES) {
+          const Pairs gt = part_load<VEC>(part_gate, j, lane, left);
+          bk.a = mul2(bk.a, gt.a); bk.b = mul2(bk.b, gt.b);
+        }
+        const Pairs e = {mul2(both(p.b), d[j].a), mul2(both(p.b), d[j].b)};
+        x[j].a = mul2(add2(h.a, pm), pr); x[j].b = mul2(add2(h.b, pm), pr);
+        A[j].a = fma2(e.a, x[j].a, A[j].a); A[j].b = fma2(e.b, x[j].b, A[j].b);
+        B[j].a = add2(B[j].a, e.a); B[j].b = add2(B[j].b, e.b);
+        d[j].a = mul2(d[j].a, bk.a); d[j].b = mul2(d[j].b, bk.b);
+        s = add2(s, add2(d[j].a, d[j].b));
+        q = fma2(d[j].a, x[j].a, q); q = fma2(d[j].b, x[j].b, q);
+      }
+    }
+    __syncwarp();                            // every lane has read its part: it takes the row after the next
+    fetch(ahead, stage);
+    if (ahead.unit < p.units) ahead.next(p, stride);
+    if (p.dh) {
+      if (post) {
+        const float2 c = team_sum_pair<WARPS>(make_float2(s.x + s.y, q.x + q.y), red, team, flip);
+        const float2 c1 = both(p.post == NORM_LAYER ? -c.x * inv_dim : 0.0f), c2 = both(-c.y * inv_dim);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+          d[j].a = mul2(pr, add2(fma2(x[j].a, c2, d[j].a), c1));
+          d[j].b = mul2(pr, add2(fma2(x[j].b, c2, d[j].b), c1));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) part_store<VEC>(p.dh + out + mine, j, left, d[j]);
+    }
+    const int unit = now.unit;
+    now.next(p, stride);
+    if (GATES && now.unit != unit) {         // the last row of a piece: what its gate gathered
+      const float* gate = p.gate + static_cast<long long>(unit / p.pieces) * p.dim;
+      float* to = (p.pieces == 1 ? p.dgate : p.gate_partial) + static_cast<long long>(unit) * p.dim + mine;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const Pairs gt = param_pairs<VEC>(gate, mine, j, left, 1.0f);
+        if (p.dgate) {
+          const Pairs pg = param_pairs<VEC>(p.post_gamma, mine, j, left, 1.0f), pb = param_pairs<VEC>(p.post_beta, mine, j, left, 0.0f);
+          part_store<VEC>(to, j, left, Pairs{fma2(pg.a, A[j].a, mul2(pb.a, B[j].a)), fma2(pg.b, A[j].b, mul2(pb.b, B[j].b))});
+        }
+        sum_post_gamma[j].a = fma2(gt.a, A[j].a, sum_post_gamma[j].a); sum_post_gamma[j].b = fma2(gt.b, A[j].b, sum_post_gamma[j].b);
+        sum_post_beta[j].a = fma2(gt.a, B[j].a, sum_post_beta[j].a); sum_post_beta[j].b = fma2(gt.b, B[j].b, sum_post_beta[j].b);
+        A[j] = B[j] = zero;
+      }
+    }
+    if (++stage == kNormStages) { stage = 0; parity ^= 1; }
+  }
+  // the block's sums: the teams' in order, through shared memory
+  auto finish = [&](int slot, const Pairs (&sum)[VPT]) {
+    if (slot < 0) return;
+    float* to = p.partial + (static_cast<long long>(blockIdx.x) * p.sums + slot) * p.dim + mine;
+    if (TEAMS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) norm_smem[(warp * VPT + j) * 32 + lane] = make_float4(sum[j].a.x, sum[j].a.y, sum[j].b.x, sum[j].b.y);
+      __syncthreads();
+      if (team > 0) return;
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      Pairs s = sum[j];
+      for (int o = 1; o < TEAMS; ++o) {
+        const float4 v = norm_smem[((o * WARPS + warp) * VPT + j) * 32 + lane];
+        s.a = add2(s.a, make_float2(v.x, v.y)); s.b = add2(s.b, make_float2(v.z, v.w));
+      }
+      part_store<VEC>(to, j, left, s);
+    }
+  };
+  finish(p.slot[SUM_GAMMA], sum_gamma);
+  finish(p.slot[SUM_BETA], sum_beta);
+  if constexpr (GATES) {
+    finish(p.slot[SUM_POST_GAMMA], sum_post_gamma);
+    finish(p.slot[SUM_POST_BETA], sum_post_beta);
+  } else {
+    Pairs s[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const Pairs pg = param_pairs<VEC>(p.post_gamma, mine, j, left, 1.0f), pb = param_pairs<VEC>(p.post_beta, mine, j, left, 0.0f);
+      s[j] = Pairs{fma2(pg.a, A[j].a, mul2(pb.a, B[j].a)), fma2(pg.b, A[j].b, mul2(pb.b, B[j].b))};
+    }
+    finish(p.slot[SUM_GATE], s);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const Pairs gt = param_pairs<VEC>(p.gate, mine, j, left, 1.0f);
+      A[j] = Pairs{mul2(gt.a, A[j].a), mul2(gt.b, A[j].b)};
+      B[j] = Pairs{mul2(gt.a, B[j].a), mul2(gt.b, B[j].b)};
+    }
+    finish(p.slot[SUM_POST_GAMMA], A);
+    finish(p.slot[SUM_POST_BETA], B);
+  }
+  if (threadIdx.x == 0 && abort_flag) atomicExch(p.error_word, 1);
+}
+
+// The backward pass of rows of 4097 to 8192 elements: a block of 16 warps a row.  The column sums are added up in shared
+// memory, where each thread keeps its own columns (five vectors of such a row do not fit beside it in registers, and a
+// second pass over the batch for them would double the traffic).
 __device__ __forceinline__ void add_to(float4* sum, const float4& v) {
   float4 s = *sum;
   s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   *sum = s;
 }
-template <int WARPS, int VPT, int VEC>
-static __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
-residual_norm_bwd_kernel(const NormGradArgs p) {
+template <int VEC>
+static __global__ void __launch_bounds__(512)
+residual_norm_bwd_long_kernel(const NormGradArgs p) {
   pdl_prologue();
-  constexpr int TEAM = 32 * WARPS, TEAMS = WARPS == 1 ? 8 : 1, VECTOR = VPT * TEAM;     // float4s of one column sum
-  extern __shared__ float4 norm_smem[];                // [TEAMS][sums (+ 1 for the gate)][VECTOR]
+  constexpr int WARPS = 16, VPT = 4, TEAM = 32 * WARPS, VECTOR = VPT * TEAM;     // float4s of one column sum
+  extern __shared__ float4 norm_smem[];                // [sums (+ 1 for the gate)][VECTOR]
   __shared__ float2 red[2][32];
   int flip = 0;
-  const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int t = threadIdx.x;
   const float inv_dim = 1.0f / p.dim;
   const int vectors = p.sums + (p.dgate != nullptr);
-  float4* const mine = norm_smem + team * vectors * VECTOR + t;
+  float4* const mine = norm_smem + t;
   float4* const gate_sum = mine + p.sums * VECTOR;
   for (int k = 0; k < vectors; ++k)
 #pragma unroll
     for (int j = 0; j < VPT; ++j) mine[k * VECTOR + j * TEAM] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int unit = blockIdx.x * TEAMS + team; unit < p.units; unit += gridDim.x * TEAMS) {
+  for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     long long row, end;
     norm_unit_rows(p, unit, &row, &end);
     const float* gate = p.gate_rows ? p.gate + static_cast<long long>(unit / p.pieces) * p.dim : nullptr;
@@ -421,12 +774,12 @@ residual_norm_bwd_kernel(const NormGradArgs p) {
         if (p.h) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) if (p.post != NORM_NONE) lane_set(h[j], k, (lane_get(h[j], k) - pm) * pr);
-          if (p.dgate) {
+          if (p.dgate || p.slot[SUM_GATE] >= 0) {
             const float4 pb = param_load<TEAM, VEC>(p.post_beta, j, t, p.dim, 0.0f);
             float4 w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) lane_set(w, k, p.b * lane_get(d[j], k) * fmaf(lane_get(h[j], k), lane_get(pg, k), lane_get(pb, k)));
-            add_to(gate_sum + j * TEAM, w);
+            add_to((p.dgate ? gate_sum : mine + p.slot[SUM_GATE] * VECTOR) + j * TEAM, w);
           }
         }
 #pragma unroll
@@ -467,21 +820,10 @@ residual_norm_bwd_kernel(const NormGradArgs p) {
       }
     }
   }
-  if (TEAMS > 1) __syncthreads();
-  // the teams' sums in order; each thread adds what lies at its own places
-  if (team == 0) {
-    for (int k = 0; k < p.sums; ++k) {
+  for (int k = 0; k < p.sums; ++k)
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        float4 s = mine[k * VECTOR + j * TEAM];
-        for (int o = 1; o < TEAMS; ++o) {
-          const float4 v = mine[(o * vectors + k) * VECTOR + j * TEAM];
-          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
-        row_store<TEAM, VEC>(p.partial + (static_cast<long long>(blockIdx.x) * p.sums + k) * p.dim, j, t, p.dim, s);
-      }
-    }
-  }
+    for (int j = 0; j < VPT; ++j)
+      row_store<TEAM, VEC>(p.partial + (static_cast<long long>(blockIdx.x) * p.sums + k) * p.dim, j, t, p.dim, mine[k * VECTOR + j * TEAM]);
 }
 
 // The column sums of all blocks, one launch for every vector: row y < sums of the grid adds vector y over the blocks'
@@ -491,7 +833,7 @@ struct NormSums {
   const float *partial, *gate_partial;
   int parts, pieces, sums, dim;
   float* out[SUM_COUNT];
-  float* gate;
+  float* gate;                   // of a gate that changes with the rows
 };
 static __global__ void __launch_bounds__(1024)
 norm_sums_kernel(const NormSums p) {

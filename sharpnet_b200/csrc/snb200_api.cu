@@ -1867,11 +1867,11 @@ extern "C" int snb200_residual_norm_fwd(snb200_handle_t h, const snb200_norm_des
 
 // How the rows of the backward pass are dealt out, from the sizes alone (the scratch size must not depend on the
 // device): units of consecutive rows that share a row of the gate, and the blocks whose teams take them in turn.
-constexpr int kNormBlocks = 296;
+constexpr int kNormBlocks = 148;
 struct NormPlan { int teams, pieces, units, blocks; };   // teams: of one block
 static NormPlan norm_plan(const snb200_norm_desc* d) {
   NormPlan n;
-  n.teams = d->dim <= 512 ? 8 : 1;
+  n.teams = d->dim <= 256 ? 16 : d->dim <= 512 ? 8 : d->dim <= 1024 ? 4 : d->dim <= 2048 ? 2 : 1;
   const long long groups = d->gate_rows > 1 ? d->gate_rows : 1, per = d->rows / groups;
   const long long all = static_cast<long long>(kNormBlocks) * n.teams;
   long long pieces = groups == 1 ? all : (2 * all + groups - 1) / groups;
@@ -1885,18 +1885,27 @@ static NormPlan norm_plan(const snb200_norm_desc* d) {
 extern "C" long long snb200_residual_norm_scratch_floats(const snb200_norm_desc* d) {
   if (!d || d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return -1;
   const NormPlan n = norm_plan(d);
-  const long long sums = 2 * (d->norm != SNB200_NORM_NONE) + 2 * (d->post_norm != SNB200_NORM_NONE);
-  return (sums * n.blocks + (d->gate_rows > 0 && n.pieces > 1 ? n.units : 0)) * d->dim;
+  const long long sums = 2 * (d->norm != SNB200_NORM_NONE) + 2 * (d->post_norm != SNB200_NORM_NONE) + (d->gate_rows == 1);
+  return (sums * n.blocks + (d->gate_rows > 1 && n.pieces > 1 ? n.units : 0)) * d->dim;
 }
 
-template <int WARPS, int VPT>
-static int launch_norm_bwd(snb200_handle_t h, const NormGradArgs& a, int blocks, bool vec) {
-  const size_t smem = static_cast<size_t>(WARPS == 1 ? 8 : 1) * (a.sums + (a.dgate ? 1 : 0)) * VPT * 32 * WARPS * sizeof(float4);
-  const auto kernel = vec ? residual_norm_bwd_kernel<WARPS, VPT, 4> : residual_norm_bwd_kernel<WARPS, VPT, 1>;
-  if (smem > 40 * 1024)   // the static part counts towards the default limit of 48 KB
-    SNB_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  launch_pdl_smem(h, kernel, dim3(blocks), dim3(WARPS == 1 ? 256 : 32 * WARPS), smem, a);
+template <typename K>
+static int launch_norm_bwd(snb200_handle_t h, K kernel, const NormGradArgs& a, int blocks, size_t smem) {
+  SNB_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  launch_pdl_smem(h, kernel, dim3(blocks), dim3(kNormThreads), smem, a);
   return 0;
+}
+template <int WARPS, int VPT>
+static int launch_norm_bwd_teams(snb200_handle_t h, const NormGradArgs& a, int blocks, bool vec) {
+  const int streams = (a.norm != NORM_NONE ? 2 : 0) + (a.dr != nullptr) + (a.h != nullptr) + (a.gate_rows > 1);
+  size_t smem = static_cast<size_t>(kNormWarps) * kNormStages * streams * norm_part<VPT>() + 2 * VPT * 512 * WARPS;
+  const size_t sums = sizeof(float4) * VPT * kNormThreads;             // where the teams' sums meet at the end
+  if (smem < sums) smem = sums;
+  if (a.gate_rows > 1)
+    return vec ? launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 4, true>, a, blocks, smem)
+               : launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 1, true>, a, blocks, smem);
+  return vec ? launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 4, false>, a, blocks, smem)
+             : launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 1, false>, a, blocks, smem);
 }
 
 extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p, const float* r,
@@ -1915,11 +1924,13 @@ extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_des
   if (!dx && !dblock && !g.gamma && !g.beta && !g.post_gamma && !g.post_beta && !g.gate)
     return fail(h, SNB200_STATUS_INVALID_VALUE, "no output is wanted");
   if (d->dim == 0) return 0;
-  float* vectors[SUM_COUNT] = {g.gamma, g.beta, g.post_gamma, g.post_beta};
+  // one gate for all rows gets its gradient like the other vectors, one that changes with the rows by its pieces
+  float* const gates = d->gate_rows > 1 ? g.gate : nullptr;
+  float* vectors[SUM_COUNT] = {g.gamma, g.beta, g.post_gamma, g.post_beta, d->gate_rows == 1 ? g.gate : nullptr};
   if (d->rows == 0) {                       // no rows: the sums are zero
     for (int k = 0; k < SUM_COUNT; ++k)
       if (vectors[k]) launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, d->dim, 256)), dim3(256), d->dim, vectors[k]);
-    if (g.gate) launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, d->dim, 256)), dim3(256), static_cast<long long>(d->gate_rows) * d->dim, g.gate);
+    if (gates) launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, d->dim, 256)), dim3(256), static_cast<long long>(d->gate_rows) * d->dim, gates);
     return check_launch(h, "residual_norm_bwd launch");
   }
   if (d->norm != SNB200_NORM_NONE && (!r || !dy || !stats)) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
@@ -1935,32 +1946,34 @@ extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_des
   a.gamma = p->gamma; a.post_gamma = p->post_gamma; a.post_beta = p->post_beta; a.gate = p->gate;
   a.r = r; a.h = (g.gate || d->post_norm != SNB200_NORM_NONE) ? block : nullptr;
   a.dy = dy; a.dr = dr; a.stats = stats; a.post_stats = post_stats; a.dx = dx; a.dh = dblock;
-  a.pieces = plan.pieces; a.units = plan.units;
+  a.pieces = plan.pieces; a.units = plan.units; a.error_word = h->error_word;
   for (int k = 0; k < SUM_COUNT; ++k) a.slot[k] = vectors[k] ? a.sums++ : -1;
-  const bool split_gate = g.gate && plan.pieces > 1;
+  const bool split_gate = gates && plan.pieces > 1;
   if ((a.sums > 0 || split_gate) && !scratch) return fail(h, SNB200_STATUS_INVALID_VALUE, "no scratch memory");
   if (!aligned16(scratch)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the scratch memory is not aligned to 16 bytes");
   a.partial = scratch;
-  a.dgate = g.gate;
+  a.dgate = gates;
   a.gate_partial = scratch + static_cast<long long>(plan.blocks) * a.sums * d->dim;
   const bool vec = d->dim % 4 == 0 && aligned16(r) && aligned16(block) && aligned16(dy) && aligned16(dr) && aligned16(dx) &&
                    aligned16(dblock) && aligned16(p->gamma) && aligned16(p->post_gamma) && aligned16(p->post_beta) &&
                    aligned16(p->gate) && (!g.gate || aligned16(g.gate));
-  if (d->dim <= 128) st = launch_norm_bwd<1, 1>(h, a, plan.blocks, vec);
-  else if (d->dim <= 256) st = launch_norm_bwd<1, 2>(h, a, plan.blocks, vec);
-  else if (d->dim <= 512) st = launch_norm_bwd<1, 4>(h, a, plan.blocks, vec);
-  else if (d->dim <= 1024) st = launch_norm_bwd<4, 2>(h, a, plan.blocks, vec);
-  else if (d->dim <= 2048) st = launch_norm_bwd<4, 4>(h, a, plan.blocks, vec);
-  else if (d->dim <= 4096) st = launch_norm_bwd<8, 4>(h, a, plan.blocks, vec);
-  else if (d->dim <= 8192) st = launch_norm_bwd<16, 4>(h, a, plan.blocks, vec);
-  else launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.blocks), dim3(256), a);
+  if (d->dim <= 128) st = launch_norm_bwd_teams<1, 1>(h, a, plan.blocks, vec);
+  else if (d->dim <= 256) st = launch_norm_bwd_teams<1, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 512) st = launch_norm_bwd_teams<2, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 1024) st = launch_norm_bwd_teams<4, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 2048) st = launch_norm_bwd_teams<8, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 4096) st = launch_norm_bwd_teams<16, 2>(h, a, plan.blocks, vec);
+  else if (d->dim <= 8192) {
+    const size_t smem = static_cast<size_t>(a.sums + (a.dgate ? 1 : 0)) * 4 * kNormThreads * sizeof(float4);
+    st = vec ? launch_norm_bwd(h, residual_norm_bwd_long_kernel<4>, a, plan.blocks, smem) : launch_norm_bwd(h, residual_norm_bwd_long_kernel<1>, a, plan.blocks, smem);
+  } else launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.blocks), dim3(256), a);
   if (st) return st;
   int launches = 1;
   if (a.sums > 0 || split_gate) {
     NormSums s;
     memset(&s, 0, sizeof(s));
     s.partial = a.partial; s.gate_partial = a.gate_partial; s.parts = plan.blocks; s.pieces = plan.pieces;
-    s.sums = a.sums; s.dim = d->dim; s.gate = g.gate;
+    s.sums = a.sums; s.dim = d->dim; s.gate = gates;
     for (int k = 0; k < SUM_COUNT; ++k)
       if (vectors[k]) s.out[a.slot[k]] = vectors[k];
     launch_pdl(h, norm_sums_kernel, dim3((d->dim + 31) / 32, a.sums + (split_gate ? d->gate_rows : 0)), dim3(1024), s);

@@ -8,6 +8,7 @@ libsharpnet_b200.so exactly as the C# P/Invoke shim does.  PyTorch is used only 
 memory; no arithmetic happens in PyTorch or on the host.
 """
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -107,7 +108,7 @@ class GPUTensor:
     def __init__(self, shape, data=None, wrapper=None, storage=None):
         self.wrapper = wrapper or GPUWrapper.FromDeviceId(0)
         self.Shape = [int(s) for s in shape]
-        count = int(np.prod(self.Shape)) if self.Shape else 1
+        count = math.prod(self.Shape)
         if storage is not None:
             assert storage.dtype == torch.float32 and storage.is_cuda and storage.is_contiguous()
             assert storage.numel() >= count
@@ -122,11 +123,11 @@ class GPUTensor:
     # -- shape helpers (Prod/Data/Tensor.cs:189,1521-1526,1645-1654) --------------------------
     @property
     def Count(self):
-        return int(np.prod(self.Shape)) if self.Shape else 1
+        return math.prod(self.Shape)
 
     @property
     def MultDim0(self):
-        return int(np.prod(self.Shape[1:])) if len(self.Shape) > 1 else 1
+        return math.prod(self.Shape[1:])
 
     @property
     def Dimension(self):

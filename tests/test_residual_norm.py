@@ -8,6 +8,7 @@ of the magnitudes.
          of m's error, which is smaller; so |gamma| (s (2 u (|t| + |m|) + (L + 1) u mean|t|) + (L / 2 + 8) u |xhat|) + 2 u |y|.
   dR:    s ((L + 8) u (|g| + mean|g| + |xhat| mean|g xhat|)) + 4 u |dR|, from the statistics given.
   column sums: at most `rows` additions of terms that are off by what dR and xhat are: (rows + 8) u sum|term| + sum E(term).
+         The gate's gradient may be taken as post_gamma sum(b dR hhat) + post_beta sum(b dR): its terms count as two each.
 y is checked on the r that the call returned, the backward pass on the statistics that it is given, so that each bound
 covers one call.  Bounds are multiplied by 1.1 for higher orders."""
 import ctypes
@@ -180,7 +181,7 @@ def _run_backward(w, rows, dim, norm, post, gate_rows, a, b, p, r, h, dy, dr, st
     from sharpnet_b200 import _capi
     up, params = _params(p, w, shift)
     guard = lambda t, s=shift: None if t is None else Guarded(t, w.device, s)  # noqa: E731
-    R, H, DY, DR, S, P = guard(r), guard(h), guard(dy), guard(dr), guard(stats, 0), guard(hstats, 0)
+    R, H, DY, DR, S, P = guard(r), guard(h), guard(dy), guard(dr), guard(stats, shift % 2), guard(hstats, shift % 2)
     wanted = ("dx", "dblock") + NAMES if wanted is None else wanted
     DX = (DR if in_place else guard(np.ones_like(r))) if "dx" in wanted else None
     DH = guard(np.ones_like(r)) if "dblock" in wanted else None
@@ -252,7 +253,7 @@ def _check_backward(w, rows, dim, norm, post, gate_rows, a, b, affine=True, bloc
             pg = 1 if p["post_gamma"] is None else d64["post_gamma"]
             pb = 0 if p["post_beta"] is None else d64["post_beta"]
             u_size = np.abs(hhat * pg) + np.abs(pb)
-            terms["gate"] = (b * dR * (hhat * pg + pb), abs(b) * (e * u_size + np.abs(dR) * (eh * np.abs(pg) + 4 * U * u_size)))
+            terms["gate"] = (np.abs(b * dR) * u_size, abs(b) * (e * u_size + np.abs(dR) * (eh * np.abs(pg) + 4 * U * u_size)))
     for name, (t, et) in terms.items():
         shape = (gate_rows, rows // gate_rows, dim) if name == "gate" else (1, rows, dim)
         n = shape[1]
