@@ -9,6 +9,7 @@
 // a chunk's border leaves a partial sum in the scratch memory, and a second launch adds those in chunk order.
 #pragma once
 #include "elementwise.cuh"
+#include "ptx.cuh"
 
 namespace snb {
 
@@ -75,23 +76,33 @@ constexpr int kSortMaxBits = 9;                      // digit of at most 9 bits:
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 
 struct SortPass {
-  const void* indices;                // the caller's indices: read by the first pass in place of keys_in
+  const void* indices;                // the caller's indices: read by the first pass in place of `in`
   int index_type, vocab, padding;
-  const unsigned *keys_in, *pos_in;
-  unsigned *keys_out, *pos_out;
+  const uint2* in;                    // (word, token)
+  uint2* out;
   unsigned *counts;                   // [bins][tiles]
   unsigned *totals;                   // [bins]
+  unsigned *present;                  // a bit per word that occurs, or NULL
   int n, tile, tiles;                 // tokens, tokens per tile (a multiple of kSortThreads)
   int shift, bits;
   int first;
   int* error_word;
 };
 
-// Key of token i: its word; `vocab` (behind every word) for padding and for indices outside the table.
-__device__ __forceinline__ unsigned sort_key(const SortPass& p, int i) {
-  if (!p.first) return p.keys_in[i];
+// Element i of a pass's input.  The first pass makes the pairs: a token's word, or `vocab` (behind every word) for padding
+// and for indices outside the table.  The others read what other blocks wrote: past the L1 cache.
+__device__ __forceinline__ uint2 sort_pair(const SortPass& p, int i) {
+  if (!p.first) return __ldcg(p.in + i);
   const int id = load_index(p.indices, p.index_type, i, p.vocab);
-  return static_cast<unsigned>((id < 0 || id == p.padding) ? p.vocab : id);
+  return make_uint2(static_cast<unsigned>((id < 0 || id == p.padding) ? p.vocab : id), static_cast<unsigned>(i));
+}
+// What the first pass notes down about token i besides.
+__device__ __forceinline__ void sort_note(const SortPass& p, int i, unsigned word) {
+  if (load_index(p.indices, p.index_type, i, p.vocab) < 0) atomicOr(p.error_word, kErrorTokenIndex);
+  if (p.present && word < static_cast<unsigned>(p.vocab)) {
+    const unsigned bit = 1u << (word & 31);
+    if (!(__ldcg(p.present + (word >> 5)) & bit)) atomicOr(p.present + (word >> 5), bit);     // frequent words ask once
+  }
 }
 
 static __global__ void __launch_bounds__(kSortThreads)
@@ -103,8 +114,9 @@ sort_count_kernel(const SortPass p) {
   __syncthreads();
   const int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
   for (int i = begin + threadIdx.x; i < end; i += kSortThreads) {
-    if (p.first && load_index(p.indices, p.index_type, i, p.vocab) < 0) atomicOr(p.error_word, kErrorTokenIndex);
-    atomicAdd(&hist[(sort_key(p, i) >> p.shift) & (bins - 1)], 1u);
+    const unsigned word = sort_pair(p, i).x;
+    if (p.first) sort_note(p, i, word);
+    atomicAdd(&hist[(word >> p.shift) & (bins - 1)], 1u);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += kSortThreads) p.counts[static_cast<size_t>(d) * p.tiles + blockIdx.x] = hist[d];
@@ -149,11 +161,17 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned* warp_s
   return before + x - v;
 }
 
-// Counts the digits of one warp's strip [begin, end) into hist (one counter per bin, the warp's own, zeroed).
+// Counts the digits of one warp's strip [begin, end) into hist (one counter per bin, the warp's own, zeroed); with NOTE
+// the first pass notes its tokens down.
+template <bool NOTE>
 __device__ __forceinline__ void sort_strip_count(const SortPass& p, int begin, int end, unsigned* hist) {
   const int lane = threadIdx.x & 31;
   const unsigned mask = (1u << p.bits) - 1;
-  for (int i = begin + lane; i < end; i += 32) atomicAdd(&hist[(sort_key(p, i) >> p.shift) & mask], 1u);
+  for (int i = begin + lane; i < end; i += 32) {
+    const unsigned word = sort_pair(p, i).x;
+    if (NOTE && p.first) sort_note(p, i, word);
+    atomicAdd(&hist[(word >> p.shift) & mask], 1u);
+  }
 }
 // Writes the pairs of the strip to their places: offset[digit] is where the strip's first pair with that digit goes.
 // Tokens are taken 32 at a time in order; lanes with the same digit take consecutive places in lane order.
@@ -163,9 +181,8 @@ __device__ __forceinline__ void sort_strip_place(const SortPass& p, int begin, i
   for (int b = begin; b < end; b += 32) {
     const int i = b + lane;
     const bool live = i < end;
-    const unsigned key = live ? sort_key(p, i) : 0;
-    const unsigned pos = live ? (p.first ? static_cast<unsigned>(i) : p.pos_in[i]) : 0;
-    const unsigned digit = live ? (key >> p.shift) & mask : 0xffffffffu;
+    const uint2 pair = live ? sort_pair(p, i) : make_uint2(0, 0);
+    const unsigned digit = live ? (pair.x >> p.shift) & mask : 0xffffffffu;
     const unsigned peers = __match_any_sync(0xffffffffu, digit);
     const unsigned rank = __popc(peers & ((1u << lane) - 1));
     unsigned to = 0;
@@ -173,7 +190,7 @@ __device__ __forceinline__ void sort_strip_place(const SortPass& p, int begin, i
     __syncwarp();
     if (live && rank == 0) offset[digit] += __popc(peers);
     __syncwarp();
-    if (live) { p.keys_out[to] = key; p.pos_out[to] = pos; }
+    if (live) p.out[to] = pair;
   }
 }
 
@@ -188,7 +205,7 @@ sort_scatter_kernel(const SortPass p) {
   const int strip = p.tile / kSortWarps;
   const int begin = min(p.n, blockIdx.x * p.tile + warp * strip);
   const int end = min(p.n, begin + strip);
-  sort_strip_count(p, begin, end, sort_smem + warp * bins);
+  sort_strip_count<false>(p, begin, end, sort_smem + warp * bins);
   __syncthreads();
   const int d = threadIdx.x;                           // bins <= kSortThreads: a thread per bin
   unsigned base = block_exclusive(d < bins ? p.totals[d] : 0, warp_sums);
@@ -202,6 +219,68 @@ sort_scatter_kernel(const SortPass p) {
   }
   __syncthreads();
   sort_strip_place(p, begin, end, sort_smem + warp * bins);
+}
+
+// The whole sort as one launch for up to 32768 tokens: one block, or a cluster of eight with a tile each.  Per pass every
+// block counts the digits of its warps' strips, the blocks read each other's counts through distributed shared memory,
+// and the pairs go to their places in global memory, which the barrier at the end of a pass makes visible to the cluster.
+// Three launches a digit cost what a small batch costs altogether (4999 tokens: 27 -> 12 us with the sums).
+constexpr int kSortClusterTokens = 32768;
+struct SortAll {
+  SortPass pass;
+  uint2 *buffer[2];
+  int passes;
+};
+static __global__ void __launch_bounds__(kSortThreads)
+sort_cluster_kernel(const SortAll all) {
+  pdl_prologue();
+  extern __shared__ unsigned sort_smem[];              // [warps][bins]
+  __shared__ unsigned counts[kSortMaxBins];            // of this block, read by the others
+  __shared__ unsigned warp_sums[kSortWarps];
+  SortPass p = all.pass;
+  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, d = threadIdx.x, rank = blockIdx.x, blocks = gridDim.x;
+  const int strip = p.tile / kSortWarps;
+  const int begin = min(p.n, rank * p.tile + warp * strip), end = min(p.n, begin + strip);
+  if (p.present) {
+    for (int i = rank * kSortThreads + d; i <= (p.vocab - 1) >> 5; i += blocks * kSortThreads) p.present[i] = 0;
+    cluster_sync_all();
+  }
+  for (int pass = 0; pass < all.passes; ++pass) {
+    p.first = pass == 0;
+    p.shift = pass * p.bits;
+    p.in = all.buffer[(pass + 1) & 1];
+    p.out = all.buffer[pass & 1];
+    for (int i = d; i < bins * kSortWarps; i += kSortThreads) sort_smem[i] = 0;
+    __syncthreads();
+    sort_strip_count<true>(p, begin, end, sort_smem + warp * bins);
+    __syncthreads();
+    unsigned sum = 0;
+    if (d < bins) {
+      for (int k = 0; k < kSortWarps; ++k) sum += sort_smem[k * bins + d];
+      counts[d] = sum;
+    }
+    cluster_sync_all();
+    unsigned before = 0, total = 0;
+    if (d < bins) {
+      for (int r = 0; r < blocks; ++r) {
+        unsigned v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(smem_u32(counts + d), r)) : "memory");
+        if (r < rank) before += v;
+        total += v;
+      }
+    }
+    unsigned base = block_exclusive(total, warp_sums) + before;
+    if (d < bins) {
+      for (int k = 0; k < kSortWarps; ++k) {
+        const unsigned c = sort_smem[k * bins + d];
+        sort_smem[k * bins + d] = base;
+        base += c;
+      }
+    }
+    __syncthreads();
+    sort_strip_place(p, begin, end, sort_smem + warp * bins);
+    cluster_sync_all();
+  }
 }
 
 // ---------------------------------------------------------------- sums over the sorted tokens
@@ -218,8 +297,10 @@ fill_zero_kernel(long long n, float* __restrict__ p) {
 }
 
 struct WordSums {
-  const unsigned *keys, *pos;         // sorted
+  const uint2* pairs;                 // (word, token), sorted
+  const unsigned* present;            // a bit per word that occurs; NULL: rows of other words are left as they are
   int n, vocab, dim, chunk, chunks, slabs;
+  long long sum_blocks;               // blocks that add rows; the others write the rows of words that do not occur
   float scale;
   int accumulate;
   const float* dy;
@@ -266,32 +347,57 @@ __device__ __forceinline__ void store_word(const WordSums& p, unsigned word, int
   store_cols<VEC>(row, slab, lane, p.dim, sum);
 }
 
+// A slab of the rows of 32 words: zeros where the word does not occur.
+template <int VEC>
+__device__ __forceinline__ void zero_words(const WordSums& p, long long id, int lane) {
+  const long long group = id / p.slabs;
+  const int slab = static_cast<int>(id % p.slabs);
+  const long long first = 32 * group;
+  if (first >= p.vocab) return;
+  const unsigned present = p.present[group];
+  const int words = static_cast<int>(min(32LL, p.vocab - first));
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (VEC == 4 && p.dim < kSlab) {                     // narrow rows: as many side by side as a warp's width holds
+    const int quads = p.dim >> 2;
+    for (int i = lane; i < words * quads; i += 32) {
+      const int w = i / quads;
+      if (!(present >> w & 1)) reinterpret_cast<float4*>(p.dtable + first * p.dim)[i] = zero;
+    }
+    return;
+  }
+  for (int w = 0; w < words; ++w)
+    if (!(present >> w & 1)) store_cols<VEC>(p.dtable + (first + w) * p.dim, slab, lane, p.dim, zero);
+}
+
 template <int VEC>
 static __global__ void __launch_bounds__(256)
 word_sums_kernel(const WordSums p) {
   pdl_prologue();
   constexpr int U = 8;                                 // rows in flight per lane
-  const long long id = blockIdx.x * 8LL + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x >= p.sum_blocks) {
+    zero_words<VEC>(p, (blockIdx.x - p.sum_blocks) * 8LL + (threadIdx.x >> 5), lane);
+    return;
+  }
+  const long long id = blockIdx.x * 8LL + (threadIdx.x >> 5);
   const int chunk = static_cast<int>(id / p.slabs), slab = static_cast<int>(id % p.slabs);
   if (chunk >= p.chunks) return;
   const int begin = chunk * p.chunk, end = min(p.n, begin + p.chunk);
   const unsigned none = 0xffffffffu, dropped = static_cast<unsigned>(p.vocab);
-  const unsigned before = begin > 0 ? p.keys[begin - 1] : none, after = end < p.n ? p.keys[end] : none;
+  const unsigned before = begin > 0 ? p.pairs[begin - 1].x : none, after = end < p.n ? p.pairs[end].x : none;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  unsigned word = p.keys[begin];
+  unsigned word = p.pairs[begin].x;
   bool entered = word == before;                       // the word began in an earlier chunk
   for (int b = begin; b < end; b += 32) {
     const int count = min(32, end - b);
-    const unsigned key = lane < count ? p.keys[b + lane] : none;
-    const unsigned pos = lane < count ? p.pos[b + lane] : 0;
+    const uint2 pair = lane < count ? p.pairs[b + lane] : make_uint2(none, 0);
     for (int j = 0; j < count; j += U) {
       float4 v[U];
       unsigned k[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        k[u] = __shfl_sync(0xffffffffu, key, (j + u) & 31);
-        const unsigned t = __shfl_sync(0xffffffffu, pos, (j + u) & 31);
+        k[u] = __shfl_sync(0xffffffffu, pair.x, (j + u) & 31);
+        const unsigned t = __shfl_sync(0xffffffffu, pair.y, (j + u) & 31);
         if (j + u >= count) k[u] = none;
         v[u] = k[u] < dropped ? load_cols<VEC>(p.dy + static_cast<long long>(t) * p.dim, slab, lane, p.dim)
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -329,14 +435,14 @@ word_join_kernel(const WordSums p) {
   const int chunk = static_cast<int>(id / p.slabs), slab = static_cast<int>(id % p.slabs);
   if (chunk + 1 >= p.chunks) return;
   const int begin = chunk * p.chunk, end = begin + p.chunk;
-  const unsigned word = p.keys[end - 1];
-  if (word >= static_cast<unsigned>(p.vocab) || p.keys[end] != word) return;          // nothing leaves this chunk
-  if (begin > 0 && p.keys[begin - 1] == word) return;                                 // it began earlier
+  const unsigned word = p.pairs[end - 1].x;
+  if (word >= static_cast<unsigned>(p.vocab) || p.pairs[end].x != word) return;          // nothing leaves this chunk
+  if (begin > 0 && p.pairs[begin - 1].x == word) return;                                 // it began earlier
   // the last chunk that the word reaches
   int last = chunk + 1;
   for (;;) {
     const long long border = static_cast<long long>(last + lane + 1) * p.chunk;       // first token of the chunk behind it
-    const bool on = border < p.n && p.keys[border] == word;
+    const bool on = border < p.n && p.pairs[border].x == word;
     const unsigned stops = __ballot_sync(0xffffffffu, !on);
     if (stops) { last += __ffs(stops) - 1; break; }
     last += 32;

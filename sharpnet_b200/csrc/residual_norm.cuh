@@ -462,7 +462,7 @@ __device__ __forceinline__ void part_store(float* row, int j, int left, const Pa
 // as a fifth stream).
 template <int WARPS, int VPT, int VEC, bool GATES>
 static __global__ void __launch_bounds__(kNormThreads, 1)
-residual_norm_bwd_kernel(const NormGradArgs p) {
+residual_norm_bwd_kernel(NormGradArgs p) {
   pdl_prologue();
   constexpr int TEAMS = kNormWarps / WARPS, COLUMNS = WARPS * VPT * 128, PART = norm_part<VPT>();
   extern __shared__ float4 norm_smem[];   // [warps][stages][streams][PART bytes], [2][COLUMNS]
@@ -482,15 +482,10 @@ residual_norm_bwd_kernel(const NormGradArgs p) {
   char* const parts = reinterpret_cast<char*>(norm_smem) + warp * kNormStages * streams * PART;
   float* const gamma = reinterpret_cast<float*>(reinterpret_cast<char*>(norm_smem) + kNormWarps * kNormStages * streams * PART);
   float* const back = gamma + COLUMNS;                                 // b gate post_gamma, or b post_gamma where the gates change
-  for (int i = threadIdx.x; i < COLUMNS; i += kNormThreads) {
-    const bool in = i < p.dim;
-    gamma[i] = !in ? 0.0f : p.gamma ? __ldg(p.gamma + i) : 1.0f;
-    const float g = !in ? 0.0f : !GATES && p.gate_rows ? p.b * __ldg(p.gate + i) : p.b;
-    back[i] = in && p.post_gamma ? g * __ldg(p.post_gamma + i) : g;
-  }
-  if (threadIdx.x < kNormWarps * kNormStages) mbar_init(&bars[0][0] + threadIdx.x, 1);
-  if (threadIdx.x == 0) { abort_flag = 0; fence_mbar_init(); }
-  __syncthreads();
+  if (lane < kNormStages) mbar_init(&bars[warp][lane], 1);          // a warp's barriers are its own
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_mbar_init();
+  __syncwarp();
 
   // lane k < streams has the warp's part of stream k copied
   const float* source = nullptr;
@@ -544,6 +539,14 @@ residual_norm_bwd_kernel(const NormGradArgs p) {
     fetch(ahead, s);
     if (ahead.unit < p.units) ahead.next(p, stride);
   }
+  // the parameters, while the first rows are on their way
+  for (int i = threadIdx.x; i < COLUMNS; i += kNormThreads) {
+    const bool in = i < p.dim;
+    gamma[i] = !in ? 0.0f : p.gamma ? __ldg(p.gamma + i) : 1.0f;
+    const float g = !in ? 0.0f : !GATES && p.gate_rows ? p.b * __ldg(p.gate + i) : p.b;
+    back[i] = in && p.post_gamma ? g * __ldg(p.post_gamma + i) : g;
+  }
+  __syncthreads();
   int stage = 0;
   unsigned parity = 0;
   while (now.unit < p.units) {
@@ -699,7 +702,7 @@ __device__ __forceinline__ void add_to(float4* sum, const float4& v) {
 }
 template <int VEC>
 static __global__ void __launch_bounds__(512)
-residual_norm_bwd_long_kernel(const NormGradArgs p) {
+residual_norm_bwd_long_kernel(NormGradArgs p) {
   pdl_prologue();
   constexpr int WARPS = 16, VPT = 4, TEAM = 32 * WARPS, VECTOR = VPT * TEAM;     // float4s of one column sum
   extern __shared__ float4 norm_smem[];                // [sums (+ 1 for the gate)][VECTOR]

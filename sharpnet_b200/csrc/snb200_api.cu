@@ -1713,19 +1713,22 @@ extern "C" int snb200_embedding_fwd(snb200_handle_t h, int index_type, long long
 // How the gradient of an embedding is cut, from its sizes alone (the scratch size must not depend on the device).
 struct EmbeddingPlan {
   int tile, tiles;             // tokens of one sorting block
+  bool cluster;                // the sort as one launch
   int passes, bits;            // digits of the sort and their width
   int chunk, chunks, slabs;    // sorted tokens of one warp of the sums; slabs of columns
-  size_t keys[2], pos[2], counts, totals, partial, bytes;   // offsets in the scratch memory
+  size_t pairs[2], counts, totals, present, partial, bytes;   // offsets in the scratch memory
 };
 static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingPlan* p) {
   if (tokens < 0 || tokens > (1ll << 30) || vocabulary < 1 || dim < 0) return false;
   const long long n = tokens;
+  p->cluster = n <= kSortClusterTokens;
   p->tiles = static_cast<int>((n + 2047) / 2048);
+  if (p->cluster) p->tiles = n <= 2048 ? 1 : 8;
   if (p->tiles > 512) p->tiles = 512;
   if (p->tiles < 1) p->tiles = 1;
   p->tile = static_cast<int>((n + p->tiles - 1) / p->tiles);
   p->tile = (p->tile + kSortThreads - 1) / kSortThreads * kSortThreads;
-  p->tiles = static_cast<int>((n + p->tile - 1) / (p->tile ? p->tile : 1));
+  if (!p->cluster) p->tiles = static_cast<int>((n + p->tile - 1) / (p->tile ? p->tile : 1));
   int key_bits = 0;
   while (key_bits < 31 && (static_cast<long long>(vocabulary) >> key_bits) != 0) ++key_bits;   // keys 0 .. vocabulary
   p->passes = (key_bits + kSortMaxBits - 1) / kSortMaxBits;
@@ -1737,7 +1740,8 @@ static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingP
   p->chunks = static_cast<int>((n + p->chunk - 1) / p->chunk);
   size_t at = 0;
   auto take = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
-  for (int k = 0; k < 2; ++k) { p->keys[k] = take(4 * static_cast<size_t>(n)); p->pos[k] = take(4 * static_cast<size_t>(n)); }
+  for (int k = 0; k < 2; ++k) p->pairs[k] = take(8 * static_cast<size_t>(n));
+  p->present = take(4 * ((static_cast<size_t>(vocabulary) + 31) / 32));
   p->counts = take(4 * static_cast<size_t>(kSortMaxBins) * p->tiles);
   p->totals = take(4 * kSortMaxBins);
   p->partial = take(8 * static_cast<size_t>(p->chunks) * dim);
@@ -1763,45 +1767,68 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
   if (!dtable || (tokens > 0 && (!indices || !dy || !scratch))) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
   if (!aligned16(scratch)) return fail(h, SNB200_STATUS_INVALID_VALUE, "the scratch memory is not aligned to 16 bytes");
   int launches = 0;
-  if (!accumulate) {
+  if (tokens == 0) {
     const long long count = static_cast<long long>(vocabulary) * dim;
     launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, count / 4 + 1, 256)), dim3(256), count, dtable);
-    ++launches;
+    note_kernel(h, "embedding_bwd", 1);
+    return check_launch(h, "embedding_bwd launch");
   }
-  if (tokens > 0) {
-    char* base = static_cast<char*>(scratch);
-    SortPass s;
-    memset(&s, 0, sizeof(s));
-    s.indices = indices; s.index_type = index_type; s.vocab = vocabulary; s.padding = padding_index;
-    s.counts = reinterpret_cast<unsigned*>(base + plan.counts);
-    s.totals = reinterpret_cast<unsigned*>(base + plan.totals);
-    s.n = static_cast<int>(tokens); s.tile = plan.tile; s.tiles = plan.tiles;
-    s.bits = plan.bits; s.error_word = h->error_word;
+  const long long sum_blocks = (static_cast<long long>(plan.chunks) * plan.slabs + 7) / 8;
+  const long long zero_blocks = accumulate ? 0 : ((static_cast<long long>(vocabulary) + 31) / 32 * plan.slabs + 7) / 8;
+  if (sum_blocks + zero_blocks > 0x7fffffffll)
+    return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
+  char* const base = static_cast<char*>(scratch);
+  uint2* const pairs[2] = {reinterpret_cast<uint2*>(base + plan.pairs[0]), reinterpret_cast<uint2*>(base + plan.pairs[1])};
+  SortPass s;
+  memset(&s, 0, sizeof(s));
+  s.indices = indices; s.index_type = index_type; s.vocab = vocabulary; s.padding = padding_index;
+  s.counts = reinterpret_cast<unsigned*>(base + plan.counts);
+  s.totals = reinterpret_cast<unsigned*>(base + plan.totals);
+  s.present = accumulate ? nullptr : reinterpret_cast<unsigned*>(base + plan.present);
+  s.n = static_cast<int>(tokens); s.tile = plan.tile; s.tiles = plan.tiles;
+  s.bits = plan.bits; s.error_word = h->error_word;
+  const size_t smem = (static_cast<size_t>(4) << plan.bits) * kSortWarps;
+  if (plan.cluster) {
+    SortAll all;
+    all.pass = s; all.buffer[0] = pairs[0]; all.buffer[1] = pairs[1]; all.passes = plan.passes;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.tiles; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(plan.tiles); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem; cfg.stream = h->stream;
+    cfg.attrs = attr; cfg.numAttrs = h->tune[TUNE_PDL] == 1 ? 1 : 2;
+    cudaLaunchKernelEx(&cfg, sort_cluster_kernel, all);
+    ++launches;
+  } else {
+    if (s.present) {
+      const long long words = (static_cast<long long>(vocabulary) + 31) / 32;
+      launch_pdl(h, fill_zero_kernel, dim3(ew_grid(h, words / 4 + 1, 256)), dim3(256), words, reinterpret_cast<float*>(s.present));
+      ++launches;
+    }
     for (int pass = 0; pass < plan.passes; ++pass) {
       s.first = pass == 0; s.shift = pass * plan.bits;
-      s.keys_in = reinterpret_cast<unsigned*>(base + plan.keys[(pass + 1) & 1]);
-      s.pos_in = reinterpret_cast<unsigned*>(base + plan.pos[(pass + 1) & 1]);
-      s.keys_out = reinterpret_cast<unsigned*>(base + plan.keys[pass & 1]);
-      s.pos_out = reinterpret_cast<unsigned*>(base + plan.pos[pass & 1]);
+      s.in = pairs[(pass + 1) & 1]; s.out = pairs[pass & 1];
       launch_pdl(h, sort_count_kernel, dim3(plan.tiles), dim3(kSortThreads), s);
       launch_pdl(h, sort_prefix_kernel, dim3(((1u << plan.bits) + 7) / 8), dim3(256), s);
-      launch_pdl_smem(h, sort_scatter_kernel, dim3(plan.tiles), dim3(kSortThreads), (static_cast<size_t>(4) << plan.bits) * kSortWarps, s);
+      launch_pdl_smem(h, sort_scatter_kernel, dim3(plan.tiles), dim3(kSortThreads), smem, s);
       launches += 3;
     }
-    WordSums w;
-    memset(&w, 0, sizeof(w));
-    w.keys = s.keys_out; w.pos = s.pos_out;
-    w.n = s.n; w.vocab = vocabulary; w.dim = dim; w.chunk = plan.chunk; w.chunks = plan.chunks; w.slabs = plan.slabs;
-    w.scale = scale; w.accumulate = accumulate ? 1 : 0; w.dy = dy; w.dtable = dtable;
-    w.partial = reinterpret_cast<float*>(base + plan.partial);
-    const long long blocks = (static_cast<long long>(plan.chunks) * plan.slabs + 7) / 8;
-    if (blocks > 0x7fffffffll) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
-    const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable);
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (vec) { launch_pdl(h, word_sums_kernel<4>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<4>, grid, dim3(256), w); }
-    else { launch_pdl(h, word_sums_kernel<1>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<1>, grid, dim3(256), w); }
-    launches += 2;
   }
+  WordSums w;
+  memset(&w, 0, sizeof(w));
+  w.pairs = pairs[(plan.passes - 1) & 1]; w.present = s.present;
+  w.n = s.n; w.vocab = vocabulary; w.dim = dim; w.chunk = plan.chunk; w.chunks = plan.chunks; w.slabs = plan.slabs;
+  w.scale = scale; w.accumulate = accumulate ? 1 : 0; w.dy = dy; w.dtable = dtable;
+  w.partial = reinterpret_cast<float*>(base + plan.partial);
+  w.sum_blocks = sum_blocks;
+  const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable);
+  const dim3 grid(static_cast<unsigned>(sum_blocks + zero_blocks)), join(static_cast<unsigned>(sum_blocks));
+  if (vec) { launch_pdl(h, word_sums_kernel<4>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<4>, join, dim3(256), w); }
+  else { launch_pdl(h, word_sums_kernel<1>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<1>, join, dim3(256), w); }
+  launches += 2;
   note_kernel(h, "embedding_bwd", launches);
   return check_launch(h, "embedding_bwd launch");
 }
@@ -1874,9 +1901,14 @@ static NormPlan norm_plan(const snb200_norm_desc* d) {
   n.teams = d->dim <= 256 ? 16 : d->dim <= 512 ? 8 : d->dim <= 1024 ? 4 : d->dim <= 2048 ? 2 : 1;
   const long long groups = d->gate_rows > 1 ? d->gate_rows : 1, per = d->rows / groups;
   const long long all = static_cast<long long>(kNormBlocks) * n.teams;
-  long long pieces = groups == 1 ? all : (2 * all + groups - 1) / groups;
-  if (pieces > per) pieces = per;
-  if (pieces < 1) pieces = 1;
+  // pieces of a group: as many as make the fewest rows in a line, a unit counting as one row more (its start and its sums)
+  long long pieces = 1, best = 0;
+  for (int waves = 1; waves <= 4; ++waves) {
+    long long k = waves * all / groups;
+    k = k > per ? per : k < 1 ? 1 : k;
+    const long long line = (groups * k + all - 1) / all * ((per + k - 1) / k + 1);
+    if (waves == 1 || line < best) { pieces = k; best = line; }
+  }
   n.pieces = static_cast<int>(pieces);
   n.units = static_cast<int>(groups * pieces);
   n.blocks = n.units < all ? (n.units + n.teams - 1) / n.teams : kNormBlocks;
@@ -1889,10 +1921,15 @@ extern "C" long long snb200_residual_norm_scratch_floats(const snb200_norm_desc*
   return (sums * n.blocks + (d->gate_rows > 1 && n.pieces > 1 ? n.units : 0)) * d->dim;
 }
 
-template <typename K>
-static int launch_norm_bwd(snb200_handle_t h, K kernel, const NormGradArgs& a, int blocks, size_t smem) {
-  SNB_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  launch_pdl_smem(h, kernel, dim3(blocks), dim3(kNormThreads), smem, a);
+// KERNEL may ask for up to 220 KB of shared memory, which has to be allowed once per device.
+template <void (*KERNEL)(NormGradArgs)>
+static int launch_norm_bwd(snb200_handle_t h, const NormGradArgs& a, int blocks, size_t smem) {
+  static bool configured[64] = {};
+  if (h->device >= 64 || !configured[h->device]) {
+    SNB_CUDA(h, cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    if (h->device < 64) configured[h->device] = true;
+  }
+  launch_pdl_smem(h, KERNEL, dim3(blocks), dim3(kNormThreads), smem, a);
   return 0;
 }
 template <int WARPS, int VPT>
@@ -1902,10 +1939,10 @@ static int launch_norm_bwd_teams(snb200_handle_t h, const NormGradArgs& a, int b
   const size_t sums = sizeof(float4) * VPT * kNormThreads;             // where the teams' sums meet at the end
   if (smem < sums) smem = sums;
   if (a.gate_rows > 1)
-    return vec ? launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 4, true>, a, blocks, smem)
-               : launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 1, true>, a, blocks, smem);
-  return vec ? launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 4, false>, a, blocks, smem)
-             : launch_norm_bwd(h, residual_norm_bwd_kernel<WARPS, VPT, 1, false>, a, blocks, smem);
+    return vec ? launch_norm_bwd<residual_norm_bwd_kernel<WARPS, VPT, 4, true>>(h, a, blocks, smem)
+               : launch_norm_bwd<residual_norm_bwd_kernel<WARPS, VPT, 1, true>>(h, a, blocks, smem);
+  return vec ? launch_norm_bwd<residual_norm_bwd_kernel<WARPS, VPT, 4, false>>(h, a, blocks, smem)
+             : launch_norm_bwd<residual_norm_bwd_kernel<WARPS, VPT, 1, false>>(h, a, blocks, smem);
 }
 
 extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p, const float* r,
@@ -1965,7 +2002,7 @@ extern "C" int snb200_residual_norm_bwd(snb200_handle_t h, const snb200_norm_des
   else if (d->dim <= 4096) st = launch_norm_bwd_teams<16, 2>(h, a, plan.blocks, vec);
   else if (d->dim <= 8192) {
     const size_t smem = static_cast<size_t>(a.sums + (a.dgate ? 1 : 0)) * 4 * kNormThreads * sizeof(float4);
-    st = vec ? launch_norm_bwd(h, residual_norm_bwd_long_kernel<4>, a, plan.blocks, smem) : launch_norm_bwd(h, residual_norm_bwd_long_kernel<1>, a, plan.blocks, smem);
+    st = vec ? launch_norm_bwd<residual_norm_bwd_long_kernel<4>>(h, a, plan.blocks, smem) : launch_norm_bwd<residual_norm_bwd_long_kernel<1>>(h, a, plan.blocks, smem);
   } else launch_pdl(h, residual_norm_bwd_wide_kernel, dim3(plan.blocks), dim3(256), a);
   if (st) return st;
   int launches = 1;
