@@ -69,244 +69,21 @@ embedding_fwd_kernel(const void* __restrict__ indices, int index_type, long long
   }
 }
 
-// ---------------------------------------------------------------- stable sort of (word, token), one digit a pass
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortMaxBits = 9;                      // digit of at most 9 bits: 16 warps x 512 counters = 32 KB
-constexpr int kSortMaxBins = 1 << kSortMaxBits;
-
-struct SortPass {
-  const void* indices;                // the caller's indices: read by the first pass in place of `in`
-  int index_type, vocab, padding;
-  const uint2* in;                    // (word, token)
-  uint2* out;
-  unsigned *counts;                   // [bins][tiles]
-  unsigned *totals;                   // [bins]
-  unsigned *present;                  // a bit per word that occurs, or NULL
-  int n, tile, tiles;                 // tokens, tokens per tile (a multiple of kSortThreads)
-  int shift, bits;
-  int first;
-  int* error_word;
-};
-
-// Element i of a pass's input.  The first pass makes the pairs: a token's word, or `vocab` (behind every word) for padding
-// and for indices outside the table.  The others read what other blocks wrote: past the L1 cache.
-__device__ __forceinline__ uint2 sort_pair(const SortPass& p, int i) {
-  if (!p.first) return __ldcg(p.in + i);
-  const int id = load_index(p.indices, p.index_type, i, p.vocab);
-  return make_uint2(static_cast<unsigned>((id < 0 || id == p.padding) ? p.vocab : id), static_cast<unsigned>(i));
-}
-// What the first pass notes down about token i besides.
-__device__ __forceinline__ void sort_note(const SortPass& p, int i, unsigned word) {
-  if (load_index(p.indices, p.index_type, i, p.vocab) < 0) atomicOr(p.error_word, kErrorTokenIndex);
-  if (p.present && word < static_cast<unsigned>(p.vocab)) {
-    const unsigned bit = 1u << (word & 31);
-    if (!(__ldcg(p.present + (word >> 5)) & bit)) atomicOr(p.present + (word >> 5), bit);     // frequent words ask once
-  }
-}
-
-static __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(const SortPass p) {
-  pdl_prologue();
-  __shared__ unsigned hist[kSortMaxBins];
-  const int bins = 1 << p.bits;
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
-  __syncthreads();
-  const int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
-  for (int i = begin + threadIdx.x; i < end; i += kSortThreads) {
-    const unsigned word = sort_pair(p, i).x;
-    if (p.first) sort_note(p, i, word);
-    atomicAdd(&hist[(word >> p.shift) & (bins - 1)], 1u);
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) p.counts[static_cast<size_t>(d) * p.tiles + blockIdx.x] = hist[d];
-}
-
-// Exclusive prefix of a bin's counts over the tiles, and its total: one warp per bin.
-static __global__ void __launch_bounds__(256)
-sort_prefix_kernel(const SortPass p) {
-  pdl_prologue();
-  const int bin = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  if (bin >= (1 << p.bits)) return;
-  unsigned* c = p.counts + static_cast<size_t>(bin) * p.tiles;
-  unsigned run = 0;
-  for (int b = 0; b < p.tiles; b += 32) {
-    const unsigned v = b + lane < p.tiles ? c[b + lane] : 0;
-    unsigned x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned up = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += up;
-    }
-    if (b + lane < p.tiles) c[b + lane] = run + x - v;
-    run += __shfl_sync(0xffffffffu, x, 31);
-  }
-  if (lane == 0) p.totals[bin] = run;
-}
-
-// Exclusive prefix sum over the kSortThreads threads of a block.
-__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned* warp_sums) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned up = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += up;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  unsigned before = 0;
-  for (int k = 0; k < warp; ++k) before += warp_sums[k];
-  __syncthreads();
-  return before + x - v;
-}
-
-// Counts the digits of one warp's strip [begin, end) into hist (one counter per bin, the warp's own, zeroed); with NOTE
-// the first pass notes its tokens down.
-template <bool NOTE>
-__device__ __forceinline__ void sort_strip_count(const SortPass& p, int begin, int end, unsigned* hist) {
-  const int lane = threadIdx.x & 31;
-  const unsigned mask = (1u << p.bits) - 1;
-  for (int i = begin + lane; i < end; i += 32) {
-    const unsigned word = sort_pair(p, i).x;
-    if (NOTE && p.first) sort_note(p, i, word);
-    atomicAdd(&hist[(word >> p.shift) & mask], 1u);
-  }
-}
-// Writes the pairs of the strip to their places: offset[digit] is where the strip's first pair with that digit goes.
-// Tokens are taken 32 at a time in order; lanes with the same digit take consecutive places in lane order.
-__device__ __forceinline__ void sort_strip_place(const SortPass& p, int begin, int end, unsigned* offset) {
-  const int lane = threadIdx.x & 31;
-  const unsigned mask = (1u << p.bits) - 1;
-  for (int b = begin; b < end; b += 32) {
-    const int i = b + lane;
-    const bool live = i < end;
-    const uint2 pair = live ? sort_pair(p, i) : make_uint2(0, 0);
-    const unsigned digit = live ? (pair.x >> p.shift) & mask : 0xffffffffu;
-    const unsigned peers = __match_any_sync(0xffffffffu, digit);
-    const unsigned rank = __popc(peers & ((1u << lane) - 1));
-    unsigned to = 0;
-    if (live) to = offset[digit] + rank;
-    __syncwarp();
-    if (live && rank == 0) offset[digit] += __popc(peers);
-    __syncwarp();
-    if (live) p.out[to] = pair;
-  }
-}
-
-static __global__ void __launch_bounds__(kSortThreads)
-sort_scatter_kernel(const SortPass p) {
-  pdl_prologue();
-  extern __shared__ unsigned sort_smem[];              // [warps][bins]
-  __shared__ unsigned warp_sums[kSortWarps];
-  const int bins = 1 << p.bits, warp = threadIdx.x >> 5;
-  for (int d = threadIdx.x; d < bins * kSortWarps; d += kSortThreads) sort_smem[d] = 0;
-  __syncthreads();
-  const int strip = p.tile / kSortWarps;
-  const int begin = min(p.n, blockIdx.x * p.tile + warp * strip);
-  const int end = min(p.n, begin + strip);
-  sort_strip_count<false>(p, begin, end, sort_smem + warp * bins);
-  __syncthreads();
-  const int d = threadIdx.x;                           // bins <= kSortThreads: a thread per bin
-  unsigned base = block_exclusive(d < bins ? p.totals[d] : 0, warp_sums);
-  if (d < bins) {
-    base += p.counts[static_cast<size_t>(d) * p.tiles + blockIdx.x];
-    for (int k = 0; k < kSortWarps; ++k) {
-      const unsigned c = sort_smem[k * bins + d];
-      sort_smem[k * bins + d] = base;
-      base += c;
-    }
-  }
-  __syncthreads();
-  sort_strip_place(p, begin, end, sort_smem + warp * bins);
-}
-
-// The whole sort as one launch for up to 32768 tokens: one block, or a cluster of eight with a tile each.  Per pass every
-// block counts the digits of its warps' strips, the blocks read each other's counts through distributed shared memory,
-// and the pairs go to their places in global memory, which the barrier at the end of a pass makes visible to the cluster.
-// Three launches a digit cost what a small batch costs altogether (4999 tokens: 27 -> 12 us with the sums).
-constexpr int kSortClusterTokens = 32768;
-struct SortAll {
-  SortPass pass;
-  uint2 *buffer[2];
-  int passes;
-};
-static __global__ void __launch_bounds__(kSortThreads)
-sort_cluster_kernel(const SortAll all) {
-  pdl_prologue();
-  extern __shared__ unsigned sort_smem[];              // [warps][bins]
-  __shared__ unsigned counts[kSortMaxBins];            // of this block, read by the others
-  __shared__ unsigned warp_sums[kSortWarps];
-  SortPass p = all.pass;
-  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, d = threadIdx.x, rank = blockIdx.x, blocks = gridDim.x;
-  const int strip = p.tile / kSortWarps;
-  const int begin = min(p.n, rank * p.tile + warp * strip), end = min(p.n, begin + strip);
-  if (p.present) {
-    for (int i = rank * kSortThreads + d; i <= (p.vocab - 1) >> 5; i += blocks * kSortThreads) p.present[i] = 0;
-    cluster_sync_all();
-  }
-  for (int pass = 0; pass < all.passes; ++pass) {
-    p.first = pass == 0;
-    p.shift = pass * p.bits;
-    p.in = all.buffer[(pass + 1) & 1];
-    p.out = all.buffer[pass & 1];
-    for (int i = d; i < bins * kSortWarps; i += kSortThreads) sort_smem[i] = 0;
-    __syncthreads();
-    sort_strip_count<true>(p, begin, end, sort_smem + warp * bins);
-    __syncthreads();
-    unsigned sum = 0;
-    if (d < bins) {
-      for (int k = 0; k < kSortWarps; ++k) sum += sort_smem[k * bins + d];
-      counts[d] = sum;
-    }
-    cluster_sync_all();
-    unsigned before = 0, total = 0;
-    if (d < bins) {
-      for (int r = 0; r < blocks; ++r) {
-        unsigned v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(smem_u32(counts + d), r)) : "memory");
-        if (r < rank) before += v;
-        total += v;
-      }
-    }
-    unsigned base = block_exclusive(total, warp_sums) + before;
-    if (d < bins) {
-      for (int k = 0; k < kSortWarps; ++k) {
-        const unsigned c = sort_smem[k * bins + d];
-        sort_smem[k * bins + d] = base;
-        base += c;
-      }
-    }
-    __syncthreads();
-    sort_strip_place(p, begin, end, sort_smem + warp * bins);
-    cluster_sync_all();
-  }
-}
-
-// ---------------------------------------------------------------- sums over the sorted tokens
-static __global__ void __launch_bounds__(256)
-fill_zero_kernel(long long n, float* __restrict__ p) {
-  pdl_prologue();
-  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long tid = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+// n floats become zero, by the threads tid = 0 .. stride - 1.
+__device__ __forceinline__ void fill_zero(long long n, float* __restrict__ p, long long tid, long long stride) {
   const long long head = min(n, static_cast<long long>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) >> 2);
   const long long quads = (n - head) >> 2;
   for (long long i = tid; i < quads; i += stride) reinterpret_cast<float4*>(p + head)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (tid < head) p[tid] = 0.0f;
   if (head + 4 * quads + tid < n) p[head + 4 * quads + tid] = 0.0f;
 }
+static __global__ void __launch_bounds__(256)
+fill_zero_kernel(long long n, float* __restrict__ p) {
+  pdl_prologue();
+  fill_zero(n, p, blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x, static_cast<long long>(gridDim.x) * blockDim.x);
+}
 
-struct WordSums {
-  const uint2* pairs;                 // (word, token), sorted
-  const unsigned* present;            // a bit per word that occurs; NULL: rows of other words are left as they are
-  int n, vocab, dim, chunk, chunks, slabs;
-  long long sum_blocks;               // blocks that add rows; the others write the rows of words that do not occur
-  float scale;
-  int accumulate;
-  const float* dy;
-  float* dtable;
-  float* partial;                     // [chunks][2][dim]: of the word that enters the chunk, of the one that leaves it
-};
+// ---------------------------------------------------------------- rows of words that do not occur
 constexpr int kSlab = 128;            // columns of one warp: 4 per lane
 
 // Four columns of a row: one float4 (VEC = 4), or the columns lane, lane + 32, .. of the slab (VEC = 1).
@@ -337,70 +114,361 @@ __device__ __forceinline__ void store_cols(float* row, int slab, int lane, int d
     if (c < dim) row[c] = lane_get(v, k);
   }
 }
-__device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
 
+// The gradient's rows of words that do not occur are zeros (unless it is added to).  Which words occur is known after the
+// first launch of the sort, so blocks that write zeros ride along with its later launches, which are bound by latency and
+// leave the memory idle.  A unit: a slab of the rows of 32 words.
+struct ZeroRows {
+  const unsigned* present;            // a bit per word that occurs
+  float* dtable;
+  int vocab, dim, slabs, vec;
+  long long first, last;              // the units of this launch
+};
 template <int VEC>
-__device__ __forceinline__ void store_word(const WordSums& p, unsigned word, int slab, int lane, float4 sum) {
-  float* row = p.dtable + static_cast<long long>(word) * p.dim;
-  sum.x *= p.scale; sum.y *= p.scale; sum.z *= p.scale; sum.w *= p.scale;
-  if (p.accumulate) add4(sum, load_cols<VEC>(row, slab, lane, p.dim));
-  store_cols<VEC>(row, slab, lane, p.dim, sum);
-}
-
-// A slab of the rows of 32 words: zeros where the word does not occur.
-template <int VEC>
-__device__ __forceinline__ void zero_words(const WordSums& p, long long id, int lane) {
-  const long long group = id / p.slabs;
-  const int slab = static_cast<int>(id % p.slabs);
+__device__ __forceinline__ void zero_words_vec(const ZeroRows& z, long long id, int lane) {
+  const long long group = id / z.slabs;
+  const int slab = static_cast<int>(id % z.slabs);
   const long long first = 32 * group;
-  if (first >= p.vocab) return;
-  const unsigned present = p.present[group];
-  const int words = static_cast<int>(min(32LL, p.vocab - first));
+  const unsigned present = __ldcg(z.present + group);
+  const int words = static_cast<int>(min(32LL, z.vocab - first));
   const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (VEC == 4 && p.dim < kSlab) {                     // narrow rows: as many side by side as a warp's width holds
-    const int quads = p.dim >> 2;
+  if (VEC == 4 && z.dim < kSlab) {                     // narrow rows: as many side by side as a warp's width holds
+    const int quads = z.dim >> 2;
     for (int i = lane; i < words * quads; i += 32) {
       const int w = i / quads;
-      if (!(present >> w & 1)) reinterpret_cast<float4*>(p.dtable + first * p.dim)[i] = zero;
+      if (!(present >> w & 1)) reinterpret_cast<float4*>(z.dtable + first * z.dim)[i] = zero;
     }
     return;
   }
   for (int w = 0; w < words; ++w)
-    if (!(present >> w & 1)) store_cols<VEC>(p.dtable + (first + w) * p.dim, slab, lane, p.dim, zero);
+    if (!(present >> w & 1)) store_cols<VEC>(z.dtable + (first + w) * z.dim, slab, lane, z.dim, zero);
+}
+// Warp `warp` of all warps that write zeros in this launch.
+__device__ __forceinline__ void zero_words(const ZeroRows& z, long long warp, long long warps) {
+  const int lane = threadIdx.x & 31;
+  for (long long id = z.first + warp; id < z.last; id += warps) {
+    if (z.vec) zero_words_vec<4>(z, id, lane);
+    else zero_words_vec<1>(z, id, lane);
+  }
 }
 
+// ---------------------------------------------------------------- stable sort of (word, token), one digit a pass
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortMaxBits = 9;                      // digit of at most 9 bits: 16 warps x 512 counters = 32 KB
+constexpr int kSortMaxBins = 1 << kSortMaxBits;
+constexpr int kSortTile = 2048;                      // tokens of a block of the sort in several launches
+constexpr int kSortClusterTokens = 32768;            // most tokens of the sort in one launch: eight blocks of 4096
+
+struct SortPass {
+  const void* indices;                // the caller's indices: read by the first pass in place of `in`
+  int index_type, vocab, padding;
+  const uint2* in;                    // (word, token)
+  uint2* out;
+  unsigned *counts;                   // [bins][tiles]
+  unsigned *totals;                   // [bins]
+  unsigned *present;                  // a bit per word that occurs, cleared before; NULL where nobody asks
+  unsigned *crossing;                 // a counter of the sums, cleared here
+  int n, tile, tiles;                 // tokens, tokens per tile (a multiple of kSortThreads)
+  int shift, bits;
+  int first;
+  int* error_word;
+};
+
+// Element i of a pass's input.  The first pass makes the pairs: a token's word, or `vocab` (behind every word) for padding
+// and for indices outside the table.  The others read what other blocks wrote: past the L1 cache.
+__device__ __forceinline__ uint2 sort_pair(const SortPass& p, int i) {
+  if (!p.first) return __ldcg(p.in + i);
+  const int id = load_index(p.indices, p.index_type, i, p.vocab);
+  if (id < 0) atomicOr(p.error_word, kErrorTokenIndex);
+  return make_uint2(static_cast<unsigned>((id < 0 || id == p.padding) ? p.vocab : id), static_cast<unsigned>(i));
+}
+
+// The words that a block's tokens name, gathered in shared memory (a frequent word asks for its bit thousands of times) and
+// handed over once, where the vocabulary's bits fit; by themselves, and only where the bit is not there yet, where not.
+constexpr int kPresentWords = 4096;                    // 131072 words: 16 KB
+__device__ __forceinline__ void present_mark(const SortPass& p, unsigned* bits, unsigned word) {
+  if (word >= static_cast<unsigned>(p.vocab)) return;
+  const unsigned bit = 1u << (word & 31);
+  if (p.vocab <= 32 * kPresentWords) {
+    if (!(bits[word >> 5] & bit)) atomicOr(bits + (word >> 5), bit);
+  } else if (!(__ldcg(p.present + (word >> 5)) & bit)) {
+    atomicOr(p.present + (word >> 5), bit);
+  }
+}
+__device__ __forceinline__ void present_clear(const SortPass& p, unsigned* bits) {
+  if (p.vocab <= 32 * kPresentWords)
+    for (int i = threadIdx.x; i <= (p.vocab - 1) >> 5; i += kSortThreads) bits[i] = 0;
+}
+__device__ __forceinline__ void present_hand_over(const SortPass& p, const unsigned* bits) {
+  if (p.vocab <= 32 * kPresentWords)
+    for (int i = threadIdx.x; i <= (p.vocab - 1) >> 5; i += kSortThreads)
+      if (bits[i]) atomicOr(p.present + i, bits[i]);
+}
+
+// A warp's strip of up to 32 * ITEMS tokens from `begin` on, in registers: token begin + 32 k + lane is item k.
+template <int ITEMS>
+__device__ __forceinline__ void sort_load(const SortPass& p, int begin, int end, uint2 (&item)[ITEMS]) {
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = begin + 32 * k + (threadIdx.x & 31);
+    if (i < end) item[k] = sort_pair(p, i);
+  }
+}
+// Counts the strip's digits in the warp's own counters (zeroed) and gives every item its rank among the items of its digit
+// that come before it in the strip: 32 at a time, lanes with the same digit in lane order.
+template <int ITEMS>
+__device__ __forceinline__ void sort_rank(const SortPass& p, int begin, int end, const uint2 (&item)[ITEMS], unsigned* hist, unsigned (&rank)[ITEMS]) {
+  const int lane = threadIdx.x & 31;
+  const unsigned mask = (1u << p.bits) - 1;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    if (begin + 32 * k >= end) break;                  // the same for the whole warp
+    const bool live = begin + 32 * k + lane < end;
+    const unsigned digit = live ? (item[k].x >> p.shift) & mask : 0xffffffffu;
+    const unsigned peers = __match_any_sync(0xffffffffu, digit);
+    const unsigned ahead = __popc(peers & ((1u << lane) - 1));
+    if (live) rank[k] = hist[digit] + ahead;
+    __syncwarp();
+    if (live && ahead == 0) hist[digit] += __popc(peers);
+    __syncwarp();
+  }
+}
+// Writes the items to their places: offset[digit] is where the strip's first item with that digit goes.
+template <int ITEMS>
+__device__ __forceinline__ void sort_place(const SortPass& p, int begin, int end, const uint2 (&item)[ITEMS], const unsigned* offset, const unsigned (&rank)[ITEMS]) {
+  const unsigned mask = (1u << p.bits) - 1;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)
+    if (begin + 32 * k + static_cast<int>(threadIdx.x & 31) < end) p.out[offset[(item[k].x >> p.shift) & mask] + rank[k]] = item[k];
+}
+
+// Exclusive prefix sum over the kSortThreads threads of a block.
+__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned* warp_sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += up;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  unsigned before = lane < warp ? warp_sums[lane & (kSortWarps - 1)] : 0;
+  before = __reduce_add_sync(0xffffffffu, before);
+  __syncthreads();
+  return before + x - v;
+}
+// The warps' counts of digit d become the places of their first items, from `base` on; returns the digit's total.
+__device__ __forceinline__ unsigned sort_total(const unsigned* smem, int bins, int d) {
+  unsigned sum = 0;
+#pragma unroll
+  for (int k = 0; k < kSortWarps; ++k) sum += smem[k * bins + d];
+  return sum;
+}
+__device__ __forceinline__ void sort_offsets(unsigned* smem, int bins, int d, unsigned base) {
+  unsigned c[kSortWarps];
+#pragma unroll
+  for (int k = 0; k < kSortWarps; ++k) c[k] = smem[k * bins + d];
+#pragma unroll
+  for (int k = 0; k < kSortWarps; ++k) { smem[k * bins + d] = base; base += c[k]; }
+}
+
+// The sort of many tokens, three launches a digit.  Counts of every tile:
+static __global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(const SortPass p) {
+  pdl_prologue();
+  constexpr int ITEMS = kSortTile / kSortThreads;
+  __shared__ unsigned hist[kSortMaxBins];
+  __shared__ unsigned bits[kPresentWords];
+  const int bins = 1 << p.bits, d = threadIdx.x;
+  const bool note = p.first && p.present;
+  if (d < bins) hist[d] = 0;
+  if (note) present_clear(p, bits);
+  if (p.first && blockIdx.x == 0 && d == 0) *p.crossing = 0;
+  uint2 item[ITEMS];
+  const int begin = blockIdx.x * p.tile + (d >> 5) * (32 * ITEMS), end = min(p.n, begin + 32 * ITEMS);
+  sort_load<ITEMS>(p, begin, end, item);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)
+    if (begin + 32 * k + (d & 31) < end) {
+      atomicAdd(&hist[(item[k].x >> p.shift) & (bins - 1)], 1u);
+      if (note) present_mark(p, bits, item[k].x);
+    }
+  __syncthreads();
+  if (d < bins) p.counts[static_cast<size_t>(d) * p.tiles + blockIdx.x] = hist[d];
+  if (note) present_hand_over(p, bits);
+}
+
+// Exclusive prefix of a bin's counts over the tiles, and its total: one warp per bin.
+static __global__ void __launch_bounds__(256)
+sort_prefix_kernel(const SortPass p) {
+  pdl_prologue();
+  const int bin = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (bin >= (1 << p.bits)) return;
+  unsigned* c = p.counts + static_cast<size_t>(bin) * p.tiles;
+  unsigned run = 0;
+  for (int b = 0; b < p.tiles; b += 32) {
+    const unsigned v = b + lane < p.tiles ? c[b + lane] : 0;
+    unsigned x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += up;
+    }
+    if (b + lane < p.tiles) c[b + lane] = run + x - v;
+    run += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) p.totals[bin] = run;
+}
+
+static __global__ void __launch_bounds__(kSortThreads)
+sort_scatter_kernel(const SortPass p, const ZeroRows z) {
+  pdl_prologue();
+  if (blockIdx.x >= p.tiles) {
+    zero_words(z, (blockIdx.x - p.tiles) * static_cast<long long>(kSortWarps) + (threadIdx.x >> 5), (gridDim.x - p.tiles) * static_cast<long long>(kSortWarps));
+    return;
+  }
+  constexpr int ITEMS = kSortTile / kSortThreads;
+  extern __shared__ unsigned sort_smem[];              // [warps][bins]
+  __shared__ unsigned warp_sums[kSortWarps];
+  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, d = threadIdx.x;     // bins <= kSortThreads: a thread per bin
+  uint2 item[ITEMS];
+  unsigned rank[ITEMS];
+  const int begin = blockIdx.x * p.tile + warp * (32 * ITEMS), end = min(p.n, begin + 32 * ITEMS);
+  sort_load<ITEMS>(p, begin, end, item);
+  const unsigned before = d < bins ? p.counts[static_cast<size_t>(d) * p.tiles + blockIdx.x] : 0;
+  const unsigned base = block_exclusive(d < bins ? p.totals[d] : 0, warp_sums) + before;
+  for (int i = d; i < bins * kSortWarps; i += kSortThreads) sort_smem[i] = 0;
+  __syncthreads();
+  sort_rank<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
+  __syncthreads();
+  if (d < bins) sort_offsets(sort_smem, bins, d, base);
+  __syncthreads();
+  sort_place<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
+}
+
+// The whole sort as one launch: one block, or a cluster of eight with a tile each.  Per pass every block ranks the items
+// of its warps' strips, the blocks read each other's counts through distributed shared memory, and the pairs go to their
+// places in global memory, which the barrier at the end of a pass makes visible to the cluster.  The other clusters of the
+// launch clear the gradient meanwhile, all of it: the rows that are summed later are few here (at most a row a token), and
+// waiting for the list of those that are not would cost more than writing them twice.
+constexpr int kSortCluster = 8;
+struct SortAll {
+  SortPass pass;
+  uint2* buffer[2];
+  int passes;
+  float* clear;                       // [zeros] floats that are set to zero
+  long long zeros;
+};
+static __global__ void __launch_bounds__(kSortThreads)
+sort_cluster_kernel(const SortAll all) {
+  pdl_prologue();
+  constexpr int ITEMS = kSortClusterTokens / kSortCluster / kSortThreads;
+  extern __shared__ unsigned sort_smem[];              // [warps][bins]
+  __shared__ unsigned counts[kSortMaxBins];            // of this block, read by the others
+  __shared__ unsigned warp_sums[kSortWarps];
+  SortPass p = all.pass;
+  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, d = threadIdx.x, here = blockIdx.x, blocks = p.tiles;
+  if (here >= blocks) {
+    fill_zero(all.zeros, all.clear, (here - blocks) * static_cast<long long>(kSortThreads) + d, (gridDim.x - blocks) * static_cast<long long>(kSortThreads));
+    return;
+  }
+  const int strip = p.tile / kSortWarps;
+  const int begin = min(p.n, here * p.tile + warp * strip), end = min(p.n, begin + strip);
+  if (here == 0 && d == 0) *p.crossing = 0;
+  uint2 item[ITEMS];
+  unsigned rank[ITEMS];
+  for (int pass = 0; pass < all.passes; ++pass) {
+    p.first = pass == 0;
+    p.shift = pass * p.bits;
+    p.in = all.buffer[(pass + 1) & 1];
+    p.out = all.buffer[pass & 1];
+    sort_load<ITEMS>(p, begin, end, item);
+    for (int i = d; i < bins * kSortWarps; i += kSortThreads) sort_smem[i] = 0;
+    __syncthreads();
+    sort_rank<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
+    __syncthreads();
+    unsigned before = 0, total = 0;
+    if (d < bins) total = counts[d] = sort_total(sort_smem, bins, d);
+    if (blocks > 1) {
+      cluster_sync_all();
+      if (d < bins) {
+        unsigned v[kSortCluster];
+#pragma unroll
+        for (int r = 0; r < kSortCluster; ++r)
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[r]) : "r"(map_to_cta(smem_u32(counts + d), r)) : "memory");
+        total = 0;
+#pragma unroll
+        for (int r = 0; r < kSortCluster; ++r) {
+          if (r < here) before += v[r];
+          total += v[r];
+        }
+      }
+    }
+    const unsigned base = block_exclusive(total, warp_sums) + before;
+    if (d < bins) sort_offsets(sort_smem, bins, d, base);
+    __syncthreads();
+    sort_place<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
+    cluster_sync_all();                                // the pairs are in place, and no block's counts are still being read
+  }
+}
+
+// ---------------------------------------------------------------- sums over the sorted tokens
+struct WordSums {
+  const uint2* pairs;                 // (word, token), sorted
+  unsigned* crossing;                 // how many words cross a border between chunks, and the chunks in which they begin
+  unsigned* crossing_chunk;
+  int n, vocab, dim, chunk, chunks, slabs;
+  float scale;
+  int accumulate;
+  const float* dy;
+  float* dtable;
+  float* partial;                     // [chunks][2][dim]: of the word that enters the chunk, of the one that leaves it
+};
+__device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+
 template <int VEC>
+__device__ __forceinline__ void store_word(const WordSums& p, unsigned word, int slab, int lane, float4 sum, const float4& old) {
+  sum.x = fmaf(p.scale, sum.x, old.x); sum.y = fmaf(p.scale, sum.y, old.y); sum.z = fmaf(p.scale, sum.z, old.z); sum.w = fmaf(p.scale, sum.w, old.w);
+  store_cols<VEC>(p.dtable + static_cast<long long>(word) * p.dim, slab, lane, p.dim, sum);
+}
+
+// A warp a chunk and slab.  U rows are in flight per lane; with ACCUMULATE the row that a word's sum is added to is fetched
+// with the word's first row, not when the sum is done (in a long tail of words that occur once that would be one memory
+// latency a row).
+template <int VEC, bool ACCUMULATE>
 static __global__ void __launch_bounds__(256)
 word_sums_kernel(const WordSums p) {
   pdl_prologue();
-  constexpr int U = 8;                                 // rows in flight per lane
+  constexpr int U = 8;
   const int lane = threadIdx.x & 31;
-  if (blockIdx.x >= p.sum_blocks) {
-    zero_words<VEC>(p, (blockIdx.x - p.sum_blocks) * 8LL + (threadIdx.x >> 5), lane);
-    return;
-  }
   const long long id = blockIdx.x * 8LL + (threadIdx.x >> 5);
   const int chunk = static_cast<int>(id / p.slabs), slab = static_cast<int>(id % p.slabs);
   if (chunk >= p.chunks) return;
   const int begin = chunk * p.chunk, end = min(p.n, begin + p.chunk);
   const unsigned none = 0xffffffffu, dropped = static_cast<unsigned>(p.vocab);
   const unsigned before = begin > 0 ? p.pairs[begin - 1].x : none, after = end < p.n ? p.pairs[end].x : none;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 sum = zero, old = zero;
   unsigned word = p.pairs[begin].x;
   bool entered = word == before;                       // the word began in an earlier chunk
+  if (ACCUMULATE && !entered && word < dropped) old = load_cols<VEC>(p.dtable + static_cast<long long>(word) * p.dim, slab, lane, p.dim);
   for (int b = begin; b < end; b += 32) {
     const int count = min(32, end - b);
     const uint2 pair = lane < count ? p.pairs[b + lane] : make_uint2(none, 0);
     for (int j = 0; j < count; j += U) {
-      float4 v[U];
+      float4 v[U], o[ACCUMULATE ? U : 1];
       unsigned k[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         k[u] = __shfl_sync(0xffffffffu, pair.x, (j + u) & 31);
         const unsigned t = __shfl_sync(0xffffffffu, pair.y, (j + u) & 31);
         if (j + u >= count) k[u] = none;
-        v[u] = k[u] < dropped ? load_cols<VEC>(p.dy + static_cast<long long>(t) * p.dim, slab, lane, p.dim)
-                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[u] = k[u] < dropped ? load_cols<VEC>(p.dy + static_cast<long long>(t) * p.dim, slab, lane, p.dim) : zero;
+        if (ACCUMULATE)
+          o[u] = k[u] < dropped && k[u] != (u ? k[u - 1] : word) ? load_cols<VEC>(p.dtable + static_cast<long long>(k[u]) * p.dim, slab, lane, p.dim) : zero;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -408,55 +476,97 @@ word_sums_kernel(const WordSums p) {
         if (k[u] != word) {                            // the word ends here
           if (word < dropped) {
             if (entered) store_cols<VEC>(p.partial + (2LL * chunk) * p.dim, slab, lane, p.dim, sum);
-            else store_word<VEC>(p, word, slab, lane, sum);
+            else store_word<VEC>(p, word, slab, lane, sum, old);
           }
           word = k[u];
           entered = false;
-          sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          sum = zero;
+          if (ACCUMULATE) old = o[u];
         }
         add4(sum, v[u]);
       }
     }
   }
   if (word >= dropped) return;
-  if (entered) store_cols<VEC>(p.partial + (2LL * chunk) * p.dim, slab, lane, p.dim, sum);
-  else if (word == after) store_cols<VEC>(p.partial + (2LL * chunk + 1) * p.dim, slab, lane, p.dim, sum);
-  else store_word<VEC>(p, word, slab, lane, sum);
+  if (entered) {
+    store_cols<VEC>(p.partial + (2LL * chunk) * p.dim, slab, lane, p.dim, sum);
+  } else if (word == after) {
+    store_cols<VEC>(p.partial + (2LL * chunk + 1) * p.dim, slab, lane, p.dim, sum);
+    if (slab == 0 && lane == 0) p.crossing_chunk[atomicAdd(p.crossing, 1u)] = static_cast<unsigned>(chunk);
+  } else {
+    store_word<VEC>(p, word, slab, lane, sum, old);
+  }
 }
 
-// The words that cross chunks: the warp of the chunk in which such a word begins adds its partial sums in chunk order.
+// The words that cross chunks.  (The order of the list does not matter: each entry is a word of its own.)  A warp takes a
+// slab of a word and adds its partial sums in chunk order; where there are many, the block's eight warps add up eight runs
+// of them, and their sums are added in order.
 template <int VEC>
 static __global__ void __launch_bounds__(256)
 word_join_kernel(const WordSums p) {
   pdl_prologue();
-  constexpr int U = 8;
-  const long long id = blockIdx.x * 8LL + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int chunk = static_cast<int>(id / p.slabs), slab = static_cast<int>(id % p.slabs);
-  if (chunk + 1 >= p.chunks) return;
-  const int begin = chunk * p.chunk, end = begin + p.chunk;
-  const unsigned word = p.pairs[end - 1].x;
-  if (word >= static_cast<unsigned>(p.vocab) || p.pairs[end].x != word) return;          // nothing leaves this chunk
-  if (begin > 0 && p.pairs[begin - 1].x == word) return;                                 // it began earlier
-  // the last chunk that the word reaches
-  int last = chunk + 1;
-  for (;;) {
-    const long long border = static_cast<long long>(last + lane + 1) * p.chunk;       // first token of the chunk behind it
-    const bool on = border < p.n && p.pairs[border].x == word;
-    const unsigned stops = __ballot_sync(0xffffffffu, !on);
-    if (stops) { last += __ffs(stops) - 1; break; }
-    last += 32;
-  }
-  float4 sum = load_cols<VEC>(p.partial + (2LL * chunk + 1) * p.dim, slab, lane, p.dim);
-  for (int j = chunk + 1; j <= last; j += U) {
-    float4 v[U];
+  constexpr int U = 8, MANY = 32;
+  __shared__ float4 run_sums[8][32];
+  __shared__ int many_last[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add_run = [&](int chunk, int slab, int from, int to) {   // partial sums [from, to) of the word that begins in `chunk`
+    float4 sum = zero;
+    for (int j = from; j < to; j += U) {
+      float4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      v[u] = j + u <= last ? load_cols<VEC>(p.partial + 2LL * (j + u) * p.dim, slab, lane, p.dim) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int u = 0; u < U; ++u)
+        v[u] = j + u < to ? load_cols<VEC>(p.partial + (2LL * (j + u) + (j + u == chunk)) * p.dim, slab, lane, p.dim) : zero;
 #pragma unroll
-    for (int u = 0; u < U; ++u) add4(sum, v[u]);
+      for (int u = 0; u < U; ++u) add4(sum, v[u]);
+    }
+    return sum;
+  };
+  auto finish = [&](int chunk, int slab, const float4& sum) {
+    const unsigned word = p.pairs[(chunk + 1LL) * p.chunk].x;
+    store_word<VEC>(p, word, slab, lane, sum, p.accumulate ? load_cols<VEC>(p.dtable + static_cast<long long>(word) * p.dim, slab, lane, p.dim) : zero);
+  };
+  const long long items = static_cast<long long>(*p.crossing) * p.slabs;
+  // neighbours in the list (the slabs of one word) go to different blocks, so that a frequent word keeps many of them busy
+  for (long long first = blockIdx.x; first < items; first += gridDim.x * 8LL) {
+    const long long item = first + static_cast<long long>(warp) * gridDim.x;
+    int last = -1;
+    if (item < items) {
+      const int chunk = static_cast<int>(p.crossing_chunk[item / p.slabs]), slab = static_cast<int>(item % p.slabs);
+      const unsigned word = p.pairs[(chunk + 1LL) * p.chunk].x;
+      last = chunk + 1;                                 // the last chunk that the word reaches
+      for (;;) {
+        const long long border = static_cast<long long>(last + lane + 1) * p.chunk;       // first token of the chunk behind it
+        const bool on = border < p.n && p.pairs[border].x == word;
+        const unsigned stops = __ballot_sync(0xffffffffu, !on);
+        if (stops) { last += __ffs(stops) - 1; break; }
+        last += 32;
+      }
+      if (last - chunk < MANY) {
+        finish(chunk, slab, add_run(chunk, slab, chunk, last + 1));
+        last = -1;
+      }
+    }
+    if (lane == 0) many_last[warp] = last;
+    __syncthreads();
+    for (int k = 0; k < 8; ++k) {
+      const int to = many_last[k];
+      if (to < 0) continue;                             // the same for the whole block
+      const long long which = first + static_cast<long long>(k) * gridDim.x;
+      const int chunk = static_cast<int>(p.crossing_chunk[which / p.slabs]), slab = static_cast<int>(which % p.slabs);
+      const int run = (to - chunk + 8) / 8, from = chunk + warp * run;
+      float4 sum = add_run(chunk, slab, from, min(to + 1, from + run));
+      run_sums[warp][lane] = sum;
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int o = 1; o < 8; ++o) add4(sum, run_sums[o][lane]);
+        finish(chunk, slab, sum);
+      }
+      __syncthreads();
+    }
+    __syncthreads();                                    // many_last has been read
   }
-  store_word<VEC>(p, word, slab, lane, sum);
 }
 
 }  // namespace snb

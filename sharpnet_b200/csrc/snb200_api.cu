@@ -1716,19 +1716,19 @@ struct EmbeddingPlan {
   bool cluster;                // the sort as one launch
   int passes, bits;            // digits of the sort and their width
   int chunk, chunks, slabs;    // sorted tokens of one warp of the sums; slabs of columns
-  size_t pairs[2], counts, totals, present, partial, bytes;   // offsets in the scratch memory
+  size_t pairs[2], present, crossing, counts, totals, partial, bytes;   // offsets in the scratch memory
 };
 static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingPlan* p) {
   if (tokens < 0 || tokens > (1ll << 30) || vocabulary < 1 || dim < 0) return false;
   const long long n = tokens;
   p->cluster = n <= kSortClusterTokens;
-  p->tiles = static_cast<int>((n + 2047) / 2048);
-  if (p->cluster) p->tiles = n <= 2048 ? 1 : 8;
-  if (p->tiles > 512) p->tiles = 512;
-  if (p->tiles < 1) p->tiles = 1;
-  p->tile = static_cast<int>((n + p->tiles - 1) / p->tiles);
-  p->tile = (p->tile + kSortThreads - 1) / kSortThreads * kSortThreads;
-  if (!p->cluster) p->tiles = static_cast<int>((n + p->tile - 1) / (p->tile ? p->tile : 1));
+  if (p->cluster) {
+    p->tiles = n <= kSortClusterTokens / kSortCluster ? 1 : kSortCluster;
+    p->tile = static_cast<int>((n + p->tiles - 1) / p->tiles + kSortThreads - 1) / kSortThreads * kSortThreads;
+  } else {
+    p->tile = kSortTile;
+    p->tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
+  }
   int key_bits = 0;
   while (key_bits < 31 && (static_cast<long long>(vocabulary) >> key_bits) != 0) ++key_bits;   // keys 0 .. vocabulary
   p->passes = (key_bits + kSortMaxBits - 1) / kSortMaxBits;
@@ -1742,7 +1742,8 @@ static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingP
   auto take = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   for (int k = 0; k < 2; ++k) p->pairs[k] = take(8 * static_cast<size_t>(n));
   p->present = take(4 * ((static_cast<size_t>(vocabulary) + 31) / 32));
-  p->counts = take(4 * static_cast<size_t>(kSortMaxBins) * p->tiles);
+  p->crossing = take(4 + 4 * static_cast<size_t>(p->chunks));
+  p->counts = take(p->cluster ? 0 : 4 * static_cast<size_t>(kSortMaxBins) * p->tiles);
   p->totals = take(4 * kSortMaxBins);
   p->partial = take(8 * static_cast<size_t>(p->chunks) * dim);
   p->bytes = at;
@@ -1774,8 +1775,7 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
     return check_launch(h, "embedding_bwd launch");
   }
   const long long sum_blocks = (static_cast<long long>(plan.chunks) * plan.slabs + 7) / 8;
-  const long long zero_blocks = accumulate ? 0 : ((static_cast<long long>(vocabulary) + 31) / 32 * plan.slabs + 7) / 8;
-  if (sum_blocks + zero_blocks > 0x7fffffffll)
+  if (sum_blocks > 0x7fffffffll)
     return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
   char* const base = static_cast<char*>(scratch);
   uint2* const pairs[2] = {reinterpret_cast<uint2*>(base + plan.pairs[0]), reinterpret_cast<uint2*>(base + plan.pairs[1])};
@@ -1784,13 +1784,28 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
   s.indices = indices; s.index_type = index_type; s.vocab = vocabulary; s.padding = padding_index;
   s.counts = reinterpret_cast<unsigned*>(base + plan.counts);
   s.totals = reinterpret_cast<unsigned*>(base + plan.totals);
-  s.present = accumulate ? nullptr : reinterpret_cast<unsigned*>(base + plan.present);
+  s.present = accumulate || plan.cluster ? nullptr : reinterpret_cast<unsigned*>(base + plan.present);
+  s.crossing = reinterpret_cast<unsigned*>(base + plan.crossing);
   s.n = static_cast<int>(tokens); s.tile = plan.tile; s.tiles = plan.tiles;
   s.bits = plan.bits; s.error_word = h->error_word;
   const size_t smem = (static_cast<size_t>(4) << plan.bits) * kSortWarps;
+  const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable);
+  ZeroRows z;
+  memset(&z, 0, sizeof(z));
+  z.present = s.present; z.dtable = dtable; z.vocab = vocabulary; z.dim = dim; z.slabs = plan.slabs; z.vec = vec;
+  const long long zero_units = accumulate ? 0 : (static_cast<long long>(vocabulary) + 31) / 32 * plan.slabs;
+  auto zero_share = [&](long long of, long long part) { z.first = zero_units * part / of; z.last = zero_units * (part + 1) / of; };
+  auto zero_blocks = [&](int warps) {           // blocks of that many warps for the launch's units
+    const long long blocks = (z.last - z.first + warps - 1) / warps, cap = 4LL * h->sm_count;
+    return static_cast<unsigned>(blocks < cap ? blocks : cap);
+  };
   if (plan.cluster) {
     SortAll all;
     all.pass = s; all.buffer[0] = pairs[0]; all.buffer[1] = pairs[1]; all.passes = plan.passes;
+    all.clear = dtable; all.zeros = accumulate ? 0 : static_cast<long long>(vocabulary) * dim;
+    // clusters that clear: a block for every 64 KB, up to two a SM
+    long long clearing = (all.zeros / 16384 + plan.tiles) / plan.tiles * (all.zeros > 0);
+    if (clearing * plan.tiles > 2 * h->sm_count) clearing = 2 * h->sm_count / plan.tiles;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr[2];
@@ -1798,7 +1813,7 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
     attr[0].val.clusterDim.x = plan.tiles; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(plan.tiles); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem; cfg.stream = h->stream;
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.tiles * (1 + clearing))); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem; cfg.stream = h->stream;
     cfg.attrs = attr; cfg.numAttrs = h->tune[TUNE_PDL] == 1 ? 1 : 2;
     cudaLaunchKernelEx(&cfg, sort_cluster_kernel, all);
     ++launches;
@@ -1810,24 +1825,31 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
     }
     for (int pass = 0; pass < plan.passes; ++pass) {
       s.first = pass == 0; s.shift = pass * plan.bits;
+      zero_share(plan.passes, pass);
       s.in = pairs[(pass + 1) & 1]; s.out = pairs[pass & 1];
       launch_pdl(h, sort_count_kernel, dim3(plan.tiles), dim3(kSortThreads), s);
       launch_pdl(h, sort_prefix_kernel, dim3(((1u << plan.bits) + 7) / 8), dim3(256), s);
-      launch_pdl_smem(h, sort_scatter_kernel, dim3(plan.tiles), dim3(kSortThreads), smem, s);
+      launch_pdl_smem(h, sort_scatter_kernel, dim3(plan.tiles + zero_blocks(kSortWarps)), dim3(kSortThreads), smem, s, z);
       launches += 3;
     }
   }
   WordSums w;
   memset(&w, 0, sizeof(w));
-  w.pairs = pairs[(plan.passes - 1) & 1]; w.present = s.present;
+  w.pairs = pairs[(plan.passes - 1) & 1]; w.crossing = s.crossing; w.crossing_chunk = s.crossing + 1;
   w.n = s.n; w.vocab = vocabulary; w.dim = dim; w.chunk = plan.chunk; w.chunks = plan.chunks; w.slabs = plan.slabs;
   w.scale = scale; w.accumulate = accumulate ? 1 : 0; w.dy = dy; w.dtable = dtable;
   w.partial = reinterpret_cast<float*>(base + plan.partial);
-  w.sum_blocks = sum_blocks;
-  const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable);
-  const dim3 grid(static_cast<unsigned>(sum_blocks + zero_blocks)), join(static_cast<unsigned>(sum_blocks));
-  if (vec) { launch_pdl(h, word_sums_kernel<4>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<4>, join, dim3(256), w); }
-  else { launch_pdl(h, word_sums_kernel<1>, grid, dim3(256), w); launch_pdl(h, word_join_kernel<1>, join, dim3(256), w); }
+  const dim3 grid(static_cast<unsigned>(sum_blocks));
+  const long long crossings = (static_cast<long long>(plan.chunks) * plan.slabs + 7) / 8, join_cap = 8LL * h->sm_count;
+  const dim3 join(static_cast<unsigned>(crossings < join_cap ? crossings : join_cap));
+#define SNB_WORD_SUMS(V)                                                              \
+  do {                                                                                \
+    if (accumulate) launch_pdl(h, word_sums_kernel<V, true>, grid, dim3(256), w);      \
+    else launch_pdl(h, word_sums_kernel<V, false>, grid, dim3(256), w);                       \
+    launch_pdl(h, word_join_kernel<V>, join, dim3(256), w);                           \
+  } while (0)
+  if (vec) SNB_WORD_SUMS(4); else SNB_WORD_SUMS(1);
+#undef SNB_WORD_SUMS
   launches += 2;
   note_kernel(h, "embedding_bwd", launches);
   return check_launch(h, "embedding_bwd launch");
