@@ -15,7 +15,7 @@ namespace snb {
 constexpr int kAdamThreads = 256;
 constexpr int kAdamChunk32 = 4096;    // elements of one work item, moments in 32 bits
 constexpr int kAdamBlock8 = 256;      // elements that share a scale, moments in 8 bits: one warp's work
-constexpr int kAdamChunk8 = 2048;     // elements of one work item, moments in 8 bits: a block per warp
+constexpr int kAdamChunk8 = 4096;     // elements of one work item, moments in 8 bits: two blocks per warp
 
 struct AdamTensor {
   const float* g;
@@ -34,20 +34,17 @@ constexpr int kAdamMaxTensors = 448;
 template <int N> struct AdamTable {
   int n;
   unsigned total;          // work items of all tensors
-  unsigned first[N];
+  unsigned first[N + 1];   // and behind the last tensor
   AdamTensor t[N];
 };
-struct AdamCoefficients { float beta1, beta2, eps, factor; };
+struct AdamCoefficients { float beta1, beta2, eps, factor, minus_zero; };
 
-// The tensor whose work items include `item`: the last one whose first item is not above it.
+// The tensor whose work items include `item`: the last one whose first item is not above it, searched from `which` on (a
+// block's items come in ascending order).
 template <int N>
-__device__ __forceinline__ int adam_find(const AdamTable<N>& table, unsigned item) {
-  int lo = 0, hi = table.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (table.first[mid] <= item) lo = mid; else hi = mid;
-  }
-  return lo;
+__device__ __forceinline__ int adam_find(const AdamTable<N>& table, unsigned item, int which) {
+  while (item >= table.first[which + 1]) ++which;
+  return which;
 }
 
 // The update of adam_one (elementwise.cuh) with its roundings written out, so that an element's result does not depend
@@ -62,8 +59,9 @@ template <int N>
 static __global__ void __launch_bounds__(kAdamThreads)
 adam_group32_kernel(const __grid_constant__ AdamTable<N> table, const AdamCoefficients c) {
   pdl_prologue();
+  int which = 0;
   for (unsigned item = blockIdx.x; item < table.total; item += gridDim.x) {
-    const int which = adam_find(table, item);
+    which = adam_find(table, item, which);
     const AdamTensor& t = table.t[which];
     const long long base = static_cast<long long>(item - table.first[which]) * kAdamChunk32;
     const int count = static_cast<int>(min(static_cast<long long>(kAdamChunk32), t.count - base));
@@ -120,98 +118,175 @@ __device__ __forceinline__ unsigned adam8_hash(unsigned x) {
   x = (x ^ (x >> 12)) * 0xB5297A4Du;
   return x ^ (x >> 15);
 }
-// r * inverse(scale), rounded at random to an e4m3 value; rnd: 20 random bits.
-__device__ __forceinline__ float adam8_round(float x, unsigned rnd) {
-  const float high = __uint_as_float((__float_as_uint(x) + rnd) & ~0xFFFFFu);
-  const float low = fmaxf(floorf(__fadd_rn(x * 512.0f, static_cast<float>(rnd) * 0x1p-20f)), 1.0f) * 0x1p-9f;
-  return x < 0x1p-6f ? (x > 0.0f ? low : 0.0f) : high;
+// r * inverse(scale) > 0, rounded at random to an e4m3 value; rnd: 20 random bits.  Below 2^-6 the values lie 2^-9 apart.
+__device__ __forceinline__ float adam8_round_low(float x, unsigned rnd) {
+  return fmaxf(floorf(__fadd_rn(x * 512.0f, static_cast<float>(rnd) * 0x1p-20f)), 1.0f) * 0x1p-9f;
 }
+__device__ __forceinline__ float adam8_round(float x, unsigned rnd) { return __uint_as_float((__float_as_uint(x) + rnd) & ~0xFFFFFu); }
 __device__ __forceinline__ float2 adam8_decode2(unsigned short codes) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(codes, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ unsigned short adam8_encode2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ unsigned adam8_encode2(float2 v) { return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3); }
+
+// A warp's block of 256 elements, and whether it can be fetched in vectors.  A warp has two blocks of an item, one after
+// the other.
+struct AdamBlock {
+  unsigned item;
+  int which;
+  long long block;
+  bool live, whole;
+  template <int N> __device__ __forceinline__ void set(const AdamTable<N>& table) {      // live and whole, from the others
+    const AdamTensor& t = table.t[which];
+    live = block * kAdamBlock8 < t.count;              // the same for the whole warp
+    whole = (t.ordinal_vec & 1) && (block + 1) * kAdamBlock8 <= t.count;
+  }
+  template <int N> __device__ __forceinline__ void start(const AdamTable<N>& table, unsigned first) {
+    item = first;
+    live = whole = false;
+    if (item >= table.total) return;
+    which = adam_find(table, item, which);
+    block = static_cast<long long>(item - table.first[which]) * (kAdamChunk8 / kAdamBlock8) + 2 * (threadIdx.x >> 5);
+    set(table);
+  }
+  template <int N> __device__ __forceinline__ void next(const AdamTable<N>& table) {
+    if (block & 1) { start(table, item + gridDim.x); return; }
+    ++block;
+    set(table);
+  }
+};
+__device__ __forceinline__ void copy_async_16(void* smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(smem))), "l"(global) : "memory");
 }
-// One element: moments in, moments and weight out; returns the root of s.
-__device__ __forceinline__ float adam8_one(const AdamCoefficients& c, float wd, float g, float& w, float& v, float r) {
-  v = __fadd_rn(__fmul_rn(c.beta1, v), __fmul_rn(1.0f - c.beta1, g));
-  const float s = __fadd_rn(__fmul_rn(c.beta2, __fmul_rn(r, r)), __fmul_rn(__fmul_rn(1.0f - c.beta2, g), g));
-  const float root = __fsqrt_rn(s);
-  w = __fsub_rn(w, __fmaf_rn(wd, w, __fdiv_rn(__fmul_rn(c.factor, v), __fadd_rn(root, c.eps))));
-  return root;
+__device__ __forceinline__ void copy_async_4(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(smem))), "l"(global) : "memory");
 }
 
+// Bound by instructions nearly as much as by memory (the 16 bytes of an element are 73 instructions' time): pairs of
+// elements go through the packed 32-bit arithmetic; the quotient of the weight's step, which no state depends on, is a
+// product with the approximate reciprocal (2 ulp); the rounding below 2^-6, which few elements need, sits behind a branch.
+// A block's elements are copied into shared memory slots of the thread that updates them while the block before them is
+// updated.
 template <int N>
-static __global__ void __launch_bounds__(kAdamThreads)
+static __global__ void __launch_bounds__(kAdamThreads, 4)
 adam_group8_kernel(const __grid_constant__ AdamTable<N> table, const AdamCoefficients c, const unsigned seed) {
   pdl_prologue();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (unsigned item = blockIdx.x; item < table.total; item += gridDim.x) {
-    const int which = adam_find(table, item);
-    const AdamTensor& t = table.t[which];
-    const long long block = static_cast<long long>(item - table.first[which]) * (kAdamChunk8 / kAdamBlock8) + warp;
-    const long long base = block * kAdamBlock8;
-    if (base >= t.count) continue;                     // the same for the whole warp
-    const float wd = t.weight_decay;
-    const float* g = t.g + base;
+  __shared__ float4 slots4[2][4][kAdamThreads];        // g, g, w, w
+  __shared__ unsigned slots1[2][4][kAdamThreads];      // codes of v, v, s, s
+  const int lane = threadIdx.x & 31;
+  // products that are added take a minus zero that the compiler does not know: it contracts packed products and sums into
+  // one operation, which would round the state once where it is defined to round twice
+  const float2 nothing = both(c.minus_zero);
+  const float2 b1 = both(c.beta1), b2 = both(c.beta2), c1 = both(1.0f - c.beta1), c2 = both(1.0f - c.beta2);
+  float scale_v = 0.0f, scale_s = 0.0f;
+  auto fetch = [&](const AdamBlock& b, int stage) {
+    if (b.live) {
+      const AdamTensor& t = table.t[b.which];
+      scale_v = t.v_scale[b.block];
+      scale_s = t.s_scale[b.block];
+      if (b.whole) {
+        const long long base = b.block * kAdamBlock8 + 4 * lane;
+        const unsigned char *v = static_cast<const unsigned char*>(t.v) + base, *s = static_cast<const unsigned char*>(t.s) + base;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          copy_async_16(&slots4[stage][j][threadIdx.x], t.g + base + 128 * j);
+          copy_async_16(&slots4[stage][2 + j][threadIdx.x], t.w + base + 128 * j);
+          copy_async_4(&slots1[stage][j][threadIdx.x], v + 128 * j);
+          copy_async_4(&slots1[stage][2 + j][threadIdx.x], s + 128 * j);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  AdamBlock ahead;
+  ahead.which = 0;
+  ahead.start(table, blockIdx.x);
+  fetch(ahead, 0);
+  for (int stage = 0; ahead.item < table.total; stage ^= 1) {
+    const AdamBlock now = ahead;
+    const float2 v_scale = both(scale_v), s_scale = both(scale_s);
+    ahead.next(table);
+    fetch(ahead, stage ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (!now.live) continue;
+    const AdamTensor& t = table.t[now.which];
+    const long long block = now.block, base = block * kAdamBlock8;
     float* w = t.w + base;
     unsigned char* vc = static_cast<unsigned char*>(t.v) + base;
     unsigned char* sc = static_cast<unsigned char*>(t.s) + base;
-    const float v_scale = t.v_scale[block], s_scale = t.s_scale[block];
-    const unsigned key = seed * 0x9E3779B1u + (t.ordinal_vec >> 1) * 0x85EB9A77u + static_cast<unsigned>(base >> 1);
+    const float2 wd = both(t.weight_decay);
+    const unsigned key = seed * 0x9E3779B1u + (t.ordinal_vec >> 1) * 0x85EB9A77u + static_cast<unsigned>(base >> 1) + 2 * lane;
     const int count = static_cast<int>(min(static_cast<long long>(kAdamBlock8), t.count - base));
-    const bool whole = (t.ordinal_vec & 1) && count == kAdamBlock8;
-    // lane's elements: 4 lane + k and 128 + 4 lane + k
-    float gv[8], wv[8], vv[8], rv[8];
+    const bool whole = now.whole;
+    // pair i of a lane: elements 128 (i / 2) + 4 lane + 2 (i % 2) and the next
+    float2 gv[4], wv[4], vv[4], rv[4];
     if (whole) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float4 a = reinterpret_cast<const float4*>(g)[32 * j + lane], b = reinterpret_cast<const float4*>(w)[32 * j + lane];
-        const unsigned vq = reinterpret_cast<const unsigned*>(vc)[32 * j + lane], sq = reinterpret_cast<const unsigned*>(sc)[32 * j + lane];
-        gv[4 * j] = a.x; gv[4 * j + 1] = a.y; gv[4 * j + 2] = a.z; gv[4 * j + 3] = a.w;
-        wv[4 * j] = b.x; wv[4 * j + 1] = b.y; wv[4 * j + 2] = b.z; wv[4 * j + 3] = b.w;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float2 p = adam8_decode2(static_cast<unsigned short>(vq >> (16 * k))), q = adam8_decode2(static_cast<unsigned short>(sq >> (16 * k)));
-          vv[4 * j + 2 * k] = p.x; vv[4 * j + 2 * k + 1] = p.y;
-          rv[4 * j + 2 * k] = q.x; rv[4 * j + 2 * k + 1] = q.y;
-        }
+        const float4 a = slots4[stage][j][threadIdx.x], b = slots4[stage][2 + j][threadIdx.x];
+        const unsigned vq = slots1[stage][j][threadIdx.x], sq = slots1[stage][2 + j][threadIdx.x];
+        gv[2 * j] = make_float2(a.x, a.y); gv[2 * j + 1] = make_float2(a.z, a.w);
+        wv[2 * j] = make_float2(b.x, b.y); wv[2 * j + 1] = make_float2(b.z, b.w);
+        vv[2 * j] = adam8_decode2(static_cast<unsigned short>(vq)); vv[2 * j + 1] = adam8_decode2(static_cast<unsigned short>(vq >> 16));
+        rv[2 * j] = adam8_decode2(static_cast<unsigned short>(sq)); rv[2 * j + 1] = adam8_decode2(static_cast<unsigned short>(sq >> 16));
       }
     } else {
+      const float* g = t.g + base;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = 128 * (i >> 2) + 4 * lane + (i & 3);
-        const bool live = e < count;
-        gv[i] = live ? g[e] : 0.0f;
-        wv[i] = live ? w[e] : 0.0f;
-        vv[i] = live ? adam8_decode2(vc[e]).x : 0.0f;
-        rv[i] = live ? adam8_decode2(sc[e]).x : 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        const int e = 128 * (i >> 1) + 4 * lane + 2 * (i & 1);
+        const bool x = e < count, y = e + 1 < count;
+        gv[i] = make_float2(x ? g[e] : 0.0f, y ? g[e + 1] : 0.0f);
+        wv[i] = make_float2(x ? w[e] : 0.0f, y ? w[e + 1] : 0.0f);
+        vv[i] = adam8_decode2(static_cast<unsigned short>((x ? vc[e] : 0u) | (y ? vc[e + 1] : 0u) << 8));
+        rv[i] = adam8_decode2(static_cast<unsigned short>((x ? sc[e] : 0u) | (y ? sc[e + 1] : 0u) << 8));
       }
     }
-    unsigned v_max = 0, r_max = 0;
+    float v_max = 0.0f;
+    unsigned r_max = 0, r_min = 0xffffffffu;           // r_min: of the bits less one, so that a zero is the largest
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      vv[i] *= v_scale;
-      rv[i] = adam8_one(c, wd, gv[i], wv[i], vv[i], rv[i] * s_scale);
-      v_max = max(v_max, __float_as_uint(vv[i]) & 0x7fffffffu);
-      r_max = max(r_max, __float_as_uint(rv[i]) & 0x7fffffffu);
+    for (int i = 0; i < 4; ++i) {
+      const float2 r = mul2(rv[i], s_scale);
+      vv[i] = add2(fma2(b1, mul2(vv[i], v_scale), nothing), fma2(c1, gv[i], nothing));
+      const float2 s = add2(fma2(b2, mul2(r, r), nothing), fma2(mul2(c2, gv[i]), gv[i], nothing));
+      rv[i] = make_float2(__fsqrt_rn(s.x), __fsqrt_rn(s.y));
+      const float2 d = add2(rv[i], both(c.eps)), n = mul2(both(c.factor), vv[i]);
+      const float2 step = fma2(wd, wv[i], make_float2(__fdividef(n.x, d.x), __fdividef(n.y, d.y)));
+      wv[i] = add2(wv[i], make_float2(-step.x, -step.y));
+      v_max = fmaxf(v_max, fmaxf(fabsf(vv[i].x), fabsf(vv[i].y)));
+      r_max = max(r_max, max(__float_as_uint(rv[i].x), __float_as_uint(rv[i].y)));
+      r_min = min(r_min, min(__float_as_uint(rv[i].x) - 1u, __float_as_uint(rv[i].y) - 1u));
     }
-    const float new_v_scale = adam8_scale(__reduce_max_sync(0xffffffffu, v_max));
-    const float new_s_scale = adam8_scale(__reduce_max_sync(0xffffffffu, r_max));
-    const float v_inv = adam8_inverse(new_v_scale), s_inv = adam8_inverse(new_s_scale);
-    unsigned vq[2] = {0, 0}, sq[2] = {0, 0};
+    r_max = __reduce_max_sync(0xffffffffu, r_max);
+    unsigned v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_max));
+    if (r_max >= 0x7f800000u) {                        // a gradient is not finite (the maximum of floats passes a NaN over)
+      unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const unsigned rnd = adam8_hash(key + static_cast<unsigned>((128 * (i >> 2) + 4 * lane + (i & 3)) >> 1));
-      const float a = adam8_round(rv[i] * s_inv, (rnd & 0xFFFFu) << 4), b = adam8_round(rv[i + 1] * s_inv, (rnd >> 16) << 4);
-      vq[i >> 2] |= static_cast<unsigned>(adam8_encode2(vv[i] * v_inv, vv[i + 1] * v_inv)) << (8 * (i & 3));
-      sq[i >> 2] |= static_cast<unsigned>(adam8_encode2(a, b)) << (8 * (i & 3));
+      for (int i = 0; i < 4; ++i) m = max(m, max(__float_as_uint(vv[i].x) & 0x7fffffffu, __float_as_uint(vv[i].y) & 0x7fffffffu));
+      v_bits = __reduce_max_sync(0xffffffffu, m);
+      r_max = 0x7f800000u;                             // (a NaN may carry its sign)
+    }
+    const float new_v_scale = adam8_scale(v_bits), new_s_scale = adam8_scale(r_max);
+    const float2 v_inv = both(adam8_inverse(new_v_scale)), s_inv = both(adam8_inverse(new_s_scale));
+    const bool low = r_min < __float_as_uint(0x1p-6f * new_s_scale) - 1u;
+    unsigned vq[2], sq[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned rnd = adam8_hash(key + 64u * (i >> 1) + (i & 1));
+      const unsigned ra = (rnd & 0xFFFFu) << 4, rb = (rnd >> 16) << 4;
+      const float2 x = mul2(rv[i], s_inv);
+      float2 y = make_float2(adam8_round(x.x, ra), adam8_round(x.y, rb));
+      if (low) {
+        if (x.x < 0x1p-6f && x.x > 0.0f) y.x = adam8_round_low(x.x, ra);
+        if (x.y < 0x1p-6f && x.y > 0.0f) y.y = adam8_round_low(x.y, rb);
+      }
+      const unsigned v = adam8_encode2(mul2(vv[i], v_inv)), s = adam8_encode2(y);
+      if (i & 1) { vq[i >> 1] |= v << 16; sq[i >> 1] |= s << 16; } else { vq[i >> 1] = v; sq[i >> 1] = s; }
     }
     if (whole) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        reinterpret_cast<float4*>(w)[32 * j + lane] = make_float4(wv[4 * j], wv[4 * j + 1], wv[4 * j + 2], wv[4 * j + 3]);
+        reinterpret_cast<float4*>(w)[32 * j + lane] = make_float4(wv[2 * j].x, wv[2 * j].y, wv[2 * j + 1].x, wv[2 * j + 1].y);
         reinterpret_cast<unsigned*>(vc)[32 * j + lane] = vq[j];
         reinterpret_cast<unsigned*>(sc)[32 * j + lane] = sq[j];
       }
@@ -220,7 +295,7 @@ adam_group8_kernel(const __grid_constant__ AdamTable<N> table, const AdamCoeffic
       for (int i = 0; i < 8; ++i) {
         const int e = 128 * (i >> 2) + 4 * lane + (i & 3);
         if (e < count) {
-          w[e] = wv[i];
+          w[e] = i & 1 ? wv[i >> 1].y : wv[i >> 1].x;
           vc[e] = static_cast<unsigned char>(vq[i >> 2] >> (8 * (i & 3)));
           sc[e] = static_cast<unsigned char>(sq[i >> 2] >> (8 * (i & 3)));
         }

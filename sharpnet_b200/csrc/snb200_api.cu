@@ -1622,8 +1622,8 @@ static int launch_adam_group(snb200_handle_t h, const snb200_adam_tensor* tensor
     if (items > 0x7fffffffull) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "more parameters than one call updates");
   }
   if (table.n == 0) return 0;
-  table.total = static_cast<unsigned>(items);
-  const unsigned cap = 8u * h->sm_count;
+  table.total = table.first[table.n] = static_cast<unsigned>(items);
+  const unsigned cap = (state_bits == 8 ? 4u : 8u) * h->sm_count;      // what is resident at a time
   const dim3 grid(table.total < cap ? table.total : cap);
   if (state_bits == 8) launch_pdl(h, adam_group8_kernel<N>, grid, dim3(kAdamThreads), table, c, seed);
   else launch_pdl(h, adam_group32_kernel<N>, grid, dim3(kAdamThreads), table, c);
@@ -1666,6 +1666,7 @@ extern "C" int snb200_adam_group_update(snb200_handle_t h, int n, const snb200_a
   const double b1p = pow(beta1, time_step), b2p = pow(beta2, time_step);
   AdamCoefficients c;
   c.factor = static_cast<float>(learning_rate * (sqrt(1.0 - b2p) / (1.0 - b1p)));
+  c.minus_zero = -0.0f;
   c.beta1 = static_cast<float>(beta1); c.beta2 = static_cast<float>(beta2); c.eps = static_cast<float>(epsilon);
   for (int next = 0; next < n && !st;)
     st = n - next <= 32 ? launch_adam_group<32>(h, tensors, &next, n, state_bits, c, weight_decay, rounding_seed)
