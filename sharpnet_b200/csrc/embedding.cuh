@@ -351,13 +351,15 @@ sort_scatter_kernel(const SortPass p, const ZeroRows z) {
 
 // The whole sort as one launch: one block, or a cluster of eight with a tile each.  Per pass every block ranks the items
 // of its warps' strips, the blocks read each other's counts through distributed shared memory, and the pairs go to their
-// places in global memory, which the barrier at the end of a pass makes visible to the cluster.  The other clusters of the
-// launch clear the gradient meanwhile, all of it: the rows that are summed later are few here (at most a row a token), and
-// waiting for the list of those that are not would cost more than writing them twice.
+// places in the blocks' shared memory, the last pass's to global memory.  The other clusters of the launch clear the
+// gradient meanwhile, all of it: the rows that are summed later are few here (at most a row a token), and waiting for the
+// list of those that are not would cost more than writing them twice.
 constexpr int kSortCluster = 8;
+constexpr int kSortClusterTile = kSortClusterTokens / kSortCluster;
 struct SortAll {
-  SortPass pass;
-  uint2* buffer[2];
+  SortPass pass;                      // tile: a power of two, 2^tile_shift
+  int tile_shift;
+  uint2* out;
   int passes;
   float* clear;                       // [zeros] floats that are set to zero
   long long zeros;
@@ -365,12 +367,13 @@ struct SortAll {
 static __global__ void __launch_bounds__(kSortThreads)
 sort_cluster_kernel(const SortAll all) {
   pdl_prologue();
-  constexpr int ITEMS = kSortClusterTokens / kSortCluster / kSortThreads;
-  extern __shared__ unsigned sort_smem[];              // [warps][bins]
+  constexpr int ITEMS = kSortClusterTile / kSortThreads;
+  extern __shared__ uint2 sort_pairs[];                // [tile] pairs, then [warps][bins] counters
   __shared__ unsigned counts[kSortMaxBins];            // of this block, read by the others
   __shared__ unsigned warp_sums[kSortWarps];
   SortPass p = all.pass;
-  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, d = threadIdx.x, here = blockIdx.x, blocks = p.tiles;
+  unsigned* const hist = reinterpret_cast<unsigned*>(sort_pairs + p.tile);
+  const int bins = 1 << p.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x, here = blockIdx.x, blocks = p.tiles;
   if (here >= blocks) {
     fill_zero(all.zeros, all.clear, (here - blocks) * static_cast<long long>(kSortThreads) + d, (gridDim.x - blocks) * static_cast<long long>(kSortThreads));
     return;
@@ -378,22 +381,27 @@ sort_cluster_kernel(const SortAll all) {
   const int strip = p.tile / kSortWarps;
   const int begin = min(p.n, here * p.tile + warp * strip), end = min(p.n, begin + strip);
   if (here == 0 && d == 0) *p.crossing = 0;
+  const unsigned mask = bins - 1, tile_mask = p.tile - 1, mine = smem_u32(sort_pairs);
   uint2 item[ITEMS];
   unsigned rank[ITEMS];
   for (int pass = 0; pass < all.passes; ++pass) {
     p.first = pass == 0;
     p.shift = pass * p.bits;
-    p.in = all.buffer[(pass + 1) & 1];
-    p.out = all.buffer[pass & 1];
-    sort_load<ITEMS>(p, begin, end, item);
-    for (int i = d; i < bins * kSortWarps; i += kSortThreads) sort_smem[i] = 0;
+    if (p.first) {
+      sort_load<ITEMS>(p, begin, end, item);
+    } else {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (begin + 32 * k + lane < end) item[k] = sort_pairs[(begin + 32 * k + lane) & tile_mask];
+    }
+    for (int i = d; i < bins * kSortWarps; i += kSortThreads) hist[i] = 0;
     __syncthreads();
-    sort_rank<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
+    sort_rank<ITEMS>(p, begin, end, item, hist + warp * bins, rank);
     __syncthreads();
     unsigned before = 0, total = 0;
-    if (d < bins) total = counts[d] = sort_total(sort_smem, bins, d);
+    if (d < bins) total = counts[d] = sort_total(hist, bins, d);
     if (blocks > 1) {
-      cluster_sync_all();
+      cluster_sync_all();                              // (and every block has its pairs in registers)
       if (d < bins) {
         unsigned v[kSortCluster];
 #pragma unroll
@@ -408,10 +416,21 @@ sort_cluster_kernel(const SortAll all) {
       }
     }
     const unsigned base = block_exclusive(total, warp_sums) + before;
-    if (d < bins) sort_offsets(sort_smem, bins, d, base);
+    if (d < bins) sort_offsets(hist, bins, d, base);
     __syncthreads();
-    sort_place<ITEMS>(p, begin, end, item, sort_smem + warp * bins, rank);
-    cluster_sync_all();                                // the pairs are in place, and no block's counts are still being read
+    if (pass + 1 == all.passes) {
+      p.out = all.out;
+      sort_place<ITEMS>(p, begin, end, item, hist + warp * bins, rank);
+    } else {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (begin + 32 * k + lane < end) {
+          const unsigned to = hist[warp * bins + ((item[k].x >> p.shift) & mask)] + rank[k];
+          const unsigned at = map_to_cta(mine + 8 * (to & tile_mask), to >> all.tile_shift);
+          asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(item[k].x), "r"(item[k].y) : "memory");
+        }
+    }
+    cluster_sync_all();                                // the pairs are in place, and no block's memory is still being used by others
   }
 }
 
@@ -439,7 +458,7 @@ __device__ __forceinline__ void store_word(const WordSums& p, unsigned word, int
 // with the word's first row, not when the sum is done (in a long tail of words that occur once that would be one memory
 // latency a row).
 template <int VEC, bool ACCUMULATE>
-static __global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256, VEC == 4 && !ACCUMULATE ? 4 : 2)
 word_sums_kernel(const WordSums p) {
   pdl_prologue();
   constexpr int U = 8;
@@ -459,26 +478,28 @@ word_sums_kernel(const WordSums p) {
     const int count = min(32, end - b);
     const uint2 pair = lane < count ? p.pairs[b + lane] : make_uint2(none, 0);
     for (int j = 0; j < count; j += U) {
+      // lanes behind the count hold `none`; j + u stays below 32 because the count is at most that and U divides 32
       float4 v[U], o[ACCUMULATE ? U : 1];
-      unsigned k[U];
+      unsigned last = word;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        k[u] = __shfl_sync(0xffffffffu, pair.x, (j + u) & 31);
-        const unsigned t = __shfl_sync(0xffffffffu, pair.y, (j + u) & 31);
-        if (j + u >= count) k[u] = none;
-        v[u] = k[u] < dropped ? load_cols<VEC>(p.dy + static_cast<long long>(t) * p.dim, slab, lane, p.dim) : zero;
-        if (ACCUMULATE)
-          o[u] = k[u] < dropped && k[u] != (u ? k[u - 1] : word) ? load_cols<VEC>(p.dtable + static_cast<long long>(k[u]) * p.dim, slab, lane, p.dim) : zero;
+        const unsigned k = __shfl_sync(0xffffffffu, pair.x, j + u), t = __shfl_sync(0xffffffffu, pair.y, j + u);
+        v[u] = k < dropped ? load_cols<VEC>(p.dy + static_cast<long long>(t) * p.dim, slab, lane, p.dim) : zero;
+        if (ACCUMULATE) {
+          o[u] = k < dropped && k != last ? load_cols<VEC>(p.dtable + static_cast<long long>(k) * p.dim, slab, lane, p.dim) : zero;
+          last = k;
+        }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (k[u] == none) continue;
-        if (k[u] != word) {                            // the word ends here
+        const unsigned k = __shfl_sync(0xffffffffu, pair.x, j + u);
+        if (k == none) break;
+        if (k != word) {                               // the word ends here
           if (word < dropped) {
             if (entered) store_cols<VEC>(p.partial + (2LL * chunk) * p.dim, slab, lane, p.dim, sum);
             else store_word<VEC>(p, word, slab, lane, sum, old);
           }
-          word = k[u];
+          word = k;
           entered = false;
           sum = zero;
           if (ACCUMULATE) old = o[u];
@@ -522,8 +543,7 @@ word_join_kernel(const WordSums p) {
     }
     return sum;
   };
-  auto finish = [&](int chunk, int slab, const float4& sum) {
-    const unsigned word = p.pairs[(chunk + 1LL) * p.chunk].x;
+  auto finish = [&](unsigned word, int slab, const float4& sum) {
     store_word<VEC>(p, word, slab, lane, sum, p.accumulate ? load_cols<VEC>(p.dtable + static_cast<long long>(word) * p.dim, slab, lane, p.dim) : zero);
   };
   const long long items = static_cast<long long>(*p.crossing) * p.slabs;
@@ -533,7 +553,10 @@ word_join_kernel(const WordSums p) {
     int last = -1;
     if (item < items) {
       const int chunk = static_cast<int>(p.crossing_chunk[item / p.slabs]), slab = static_cast<int>(item % p.slabs);
+      // most words reach one chunk behind their first: what depends on the chunk alone is fetched together
       const unsigned word = p.pairs[(chunk + 1LL) * p.chunk].x;
+      const float4 begun = load_cols<VEC>(p.partial + (2LL * chunk + 1) * p.dim, slab, lane, p.dim);
+      const float4 behind = load_cols<VEC>(p.partial + (2LL * chunk + 2) * p.dim, slab, lane, p.dim);
       last = chunk + 1;                                 // the last chunk that the word reaches
       for (;;) {
         const long long border = static_cast<long long>(last + lane + 1) * p.chunk;       // first token of the chunk behind it
@@ -543,7 +566,10 @@ word_join_kernel(const WordSums p) {
         last += 32;
       }
       if (last - chunk < MANY) {
-        finish(chunk, slab, add_run(chunk, slab, chunk, last + 1));
+        float4 sum = begun;
+        add4(sum, behind);
+        if (last > chunk + 1) add4(sum, add_run(chunk, slab, chunk + 2, last + 1));
+        finish(word, slab, sum);
         last = -1;
       }
     }
@@ -561,7 +587,7 @@ word_join_kernel(const WordSums p) {
       if (warp == 0) {
 #pragma unroll
         for (int o = 1; o < 8; ++o) add4(sum, run_sums[o][lane]);
-        finish(chunk, slab, sum);
+        finish(p.pairs[(chunk + 1LL) * p.chunk].x, slab, sum);
       }
       __syncthreads();
     }

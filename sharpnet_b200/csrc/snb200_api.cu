@@ -1724,8 +1724,9 @@ static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingP
   const long long n = tokens;
   p->cluster = n <= kSortClusterTokens;
   if (p->cluster) {
-    p->tiles = n <= kSortClusterTokens / kSortCluster ? 1 : kSortCluster;
-    p->tile = static_cast<int>((n + p->tiles - 1) / p->tiles + kSortThreads - 1) / kSortThreads * kSortThreads;
+    p->tiles = n <= kSortClusterTile ? 1 : kSortCluster;
+    p->tile = kSortThreads;                          // a power of two: the sort finds an item's block by a shift
+    while (static_cast<long long>(p->tile) * p->tiles < n) p->tile *= 2;
   } else {
     p->tile = kSortTile;
     p->tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
@@ -1801,8 +1802,16 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
     return static_cast<unsigned>(blocks < cap ? blocks : cap);
   };
   if (plan.cluster) {
+    static bool configured[64] = {};
+    if (h->device >= 64 || !configured[h->device]) {
+      SNB_CUDA(h, cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       8 * kSortClusterTile + 4 * kSortMaxBins * kSortWarps));
+      if (h->device < 64) configured[h->device] = true;
+    }
     SortAll all;
-    all.pass = s; all.buffer[0] = pairs[0]; all.buffer[1] = pairs[1]; all.passes = plan.passes;
+    all.pass = s; all.out = pairs[(plan.passes - 1) & 1]; all.passes = plan.passes;
+    all.tile_shift = 0;
+    while (1 << all.tile_shift < plan.tile) ++all.tile_shift;
     all.clear = dtable; all.zeros = accumulate ? 0 : static_cast<long long>(vocabulary) * dim;
     // clusters that clear: a block for every 64 KB, up to two a SM
     long long clearing = (all.zeros / 16384 + plan.tiles) / plan.tiles * (all.zeros > 0);
@@ -1814,7 +1823,7 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
     attr[0].val.clusterDim.x = plan.tiles; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(plan.tiles * (1 + clearing))); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem; cfg.stream = h->stream;
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.tiles * (1 + clearing))); cfg.blockDim = dim3(kSortThreads); cfg.dynamicSmemBytes = smem + 8 * static_cast<size_t>(plan.tile); cfg.stream = h->stream;
     cfg.attrs = attr; cfg.numAttrs = h->tune[TUNE_PDL] == 1 ? 1 : 2;
     cudaLaunchKernelEx(&cfg, sort_cluster_kernel, all);
     ++launches;
