@@ -363,7 +363,8 @@ int snb200_adam_update(snb200_handle_t handle, long long count, double learning_
 
 /* The same Adam / AdamW update for ALL tensors of a model in one launch (up to 448 tensors per launch): what the loop
  * of Network.UpdateWeights over the layers' Adam.UpdateWeights (Prod/Optimizers/Adam.cs:59-72) issues tensor by tensor.
- * Element for element the formula of snb200_adam_update (last bits may differ), with weight_decay * decay of the tensor in place of
+ * Element for element the formula of snb200_adam_update, in 32 bits with the rates rounded to 32 bits as there (last bits
+ * may differ), with weight_decay * decay of the tensor in place of
  * weight_decay (decay 0 for biases and norms is customary).
  * state_bits 32: adam_vW and adam_sW are float arrays of `count` elements; the scales are not read.
  * state_bits 8: they are byte arrays of `count` elements, and v_scale and s_scale hold one float per 256 consecutive

@@ -27,7 +27,8 @@ class EmbeddingLayer:
     """y[t, :] = scale * Weights[x[t], :], and its gradient.
 
     ``paddingIndex``: tokens with this index receive no gradient (-1: none).  ``weights`` / ``weightGradients`` are
-    tensors of shape [vocabularySize, embeddingDim] to use in place of new ones (a table shared with another layer).
+    tensors of shape [vocabularySize, embeddingDim] to use in place of new ones of zeros (a table shared with another
+    layer).  Make the first pass, which allocates, before capturing a graph.
     The scratch memory of the backward pass belongs to the layer: passes of one layer that may run at the same time on
     the GPU (two streams, two captured graphs) need a layer each."""
 
@@ -39,18 +40,23 @@ class EmbeddingLayer:
             if t is not None and list(t.Shape) != shape:
                 raise ValueError(f"the table must be {shape}, not {t.Shape}")
         self._weights, self._weightGradients = weights, weightGradients
-        self._scratch = None
+        self._scratch = []          # the last one is in use; kernels queued earlier may still read the others
+
+    def _new_table(self):
+        t = GPUTensor((self.vocabularySize, self.embeddingDim), None, self.w)
+        torch.cuda.current_stream(self.w.device).synchronize()      # its zeros, before the handle's stream reads it
+        return t
 
     @property
     def Weights(self):
         if self._weights is None:
-            self._weights = GPUTensor((self.vocabularySize, self.embeddingDim), None, self.w)
+            self._weights = self._new_table()
         return self._weights
 
     @property
     def WeightGradients(self):
         if self._weightGradients is None:
-            self._weightGradients = GPUTensor((self.vocabularySize, self.embeddingDim), None, self.w)
+            self._weightGradients = self._new_table()
         return self._weightGradients
 
     def ForwardPropagation(self, x, y):
@@ -69,9 +75,8 @@ class EmbeddingLayer:
         if dy.Count != tokens * self.embeddingDim:
             raise ValueError(f"dy must hold {tokens} x {self.embeddingDim} elements, not {dy.Shape}")
         need = w.lib.snb200_embedding_scratch_bytes(tokens, self.vocabularySize, self.embeddingDim)
-        if need > 0 and (self._scratch is None or self._scratch.numel() < need):
-            self._scratch = torch.empty(need, dtype=torch.uint8, device=w.device)
+        if not self._scratch or self._scratch[-1].numel() < need:
+            self._scratch.append(torch.empty(max(need, 16), dtype=torch.uint8, device=w.device))
         check(w.handle, w.lib.snb200_embedding_bwd(
             w.handle, kind, tokens, self.vocabularySize, self.embeddingDim, at, self.scale, self.paddingIndex, int(bool(accumulate)),
-            dy.storage.data_ptr(), None if self._scratch is None else self._scratch.data_ptr(),
-            self.WeightGradients.storage.data_ptr()))
+            dy.storage.data_ptr(), self._scratch[-1].data_ptr(), self.WeightGradients.storage.data_ptr()))

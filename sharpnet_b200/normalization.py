@@ -24,7 +24,8 @@ class ResidualNorm:
     [gate_rows, dim].  By default a norm has a gamma of ones, a LayerNorm a beta of zeros as well, and a gate is ones;
     ``parameters`` / ``gradients`` replace all of them (None: the parameter is not there, the gradient is not wanted).
     The statistics of the forward pass and the scratch memory of the backward pass belong to the layer: passes of one
-    layer that may run at the same time on the GPU (two streams, two captured graphs) need a layer each."""
+    layer that may run at the same time on the GPU (two streams, two captured graphs) need a layer each.  Make the first
+    passes, which allocate, before capturing a graph."""
 
     def __init__(self, dim, wrapper, norm="layer", post_norm="none", gate_rows=0, residual_scale=1.0, block_scale=1.0,
                  epsilon=1e-5, parameters=None, gradients=None):
@@ -48,7 +49,10 @@ class ResidualNorm:
             for p, t in tensors.items():
                 if t is not None and t.Count != shapes[p][0] * self.dim:
                     raise ValueError(f"{p} must hold {shapes[p]} elements, not {t.Shape}")
-        self._stats = self._post_stats = self._scratch = None
+        self._stats = self._post_stats = None
+        self._kept = []             # buffers that were outgrown: kernels queued earlier may still use them
+        self._scratch = None
+        torch.cuda.current_stream(wrapper.device).synchronize()     # what was filled above, before the handle's stream reads it
 
     def SetStatistics(self, stats, post_stats):
         """The [rows, 2] tensors that the forward pass writes and the backward pass reads (new ones by default)."""
@@ -57,6 +61,10 @@ class ResidualNorm:
     @staticmethod
     def _structure(tensors):
         return _capi.NormParams(*[_at(tensors[p]) for p in _PARAMETERS])
+
+    def _buffer(self, count, shape):
+        self._kept.append(GPUTensor(shape, None, self.w, torch.empty(max(count, 4), dtype=torch.float32, device=self.w.device)))
+        return self._kept[-1]
 
     def _rows(self, **tensors):
         count = None
@@ -76,9 +84,9 @@ class ResidualNorm:
         """``block`` None: a norm alone; ``r`` may then be None, and may always be ``x``."""
         w, rows = self.w, self._rows(x=x, block=block, r=r, y=y)
         if self._desc.norm and (self._stats is None or self._stats.Count < 2 * rows):
-            self._stats = GPUTensor((rows, 2), None, w)
+            self._stats = self._buffer(2 * rows, (rows, 2))
         if self._desc.post_norm and (self._post_stats is None or self._post_stats.Count < 2 * rows):
-            self._post_stats = GPUTensor((rows, 2), None, w)
+            self._post_stats = self._buffer(2 * rows, (rows, 2))
         check(w.handle, w.lib.snb200_residual_norm_fwd(w.handle, self._desc, self._structure(self.Parameters), _at(x), _at(block),
                                                        _at(r), _at(y), _at(self._stats), _at(self._post_stats)))
 
@@ -90,9 +98,9 @@ class ResidualNorm:
             if needed and (stats is None or stats.Count < 2 * rows):
                 raise ValueError("no statistics of a forward pass over these rows")
         need = w.lib.snb200_residual_norm_scratch_floats(self._desc)
-        if need > 0 and (self._scratch is None or self._scratch.numel() < need):
-            self._scratch = torch.empty(need, dtype=torch.float32, device=w.device)
+        if self._scratch is None or self._scratch.Count < need:
+            self._scratch = self._buffer(need, (need,))
         check(w.handle, w.lib.snb200_residual_norm_bwd(
             w.handle, self._desc, self._structure(self.Parameters), _at(r), _at(block), _at(dy), _at(dr), _at(self._stats),
-            _at(self._post_stats), None if self._scratch is None else self._scratch.data_ptr(), _at(dx), _at(dblock),
+            _at(self._post_stats), _at(self._scratch), _at(dx), _at(dblock),
             self._structure(self.Gradients)))

@@ -92,9 +92,10 @@ class AdamGroup:
             blocks = -(-t.Count // 256)
             if ([p.numel() for p in s] != [t.Count] * 2 + ([blocks] * 2 if state_bits == 8 else []) or
                     any(not p.is_contiguous() or p.device != wrapper.device for p in s) or
-                    any(p.element_size() != (1 if state_bits == 8 else 4) for p in s[:2]) or
+                    any(p.element_size() != 1 if state_bits == 8 else p.dtype != torch.float32 for p in s[:2]) or
                     any(p.dtype != torch.float32 for p in s[2:])):
                 raise ValueError(f"the moments do not match a weight tensor of {t.Count} elements")
+        torch.cuda.current_stream(wrapper.device).synchronize()      # the zeros above, before the handle's stream reads them
         self._tensors, self.states = (list(weights), list(weightGradients)), list(states)
         self._table = (_capi.AdamTensor * len(weights))(*[
             _capi.AdamTensor(t.Count, g.storage.data_ptr(), t.storage.data_ptr(), *[p.data_ptr() for p in s],
