@@ -405,7 +405,8 @@ int snb200_embedding_fwd(snb200_handle_t handle, int index_type, long long token
  * padding_index (-1: none) and tokens whose index lies outside the table contribute nothing; the latter are reported
  * like those of the forward call.  With accumulate, rows of words that do not occur are left as they are.
  * `scratch` is caller-provided device memory of at least snb200_embedding_scratch_bytes(tokens, vocabulary, dim) bytes,
- * 16-byte aligned (-1: invalid sizes); calls that may run at the same time need one each.  At most 2^30 tokens. */
+ * 16-byte aligned (-1: invalid sizes); calls that may run at the same time need one each.  At most 2^30 tokens, and rows
+ * of at most 2^24 elements in both directions (NOT_SUPPORTED beyond). */
 long long snb200_embedding_scratch_bytes(long long tokens, int vocabulary, int dim);
 int snb200_embedding_bwd(snb200_handle_t handle, int index_type, long long tokens, int vocabulary, int dim,
                          const void* indices, float scale, int padding_index, int accumulate, const float* dy,
@@ -423,7 +424,7 @@ int snb200_embedding_bwd(snb200_handle_t handle, int index_type, long long token
  *   block NULL: r = residual_scale * x (a norm alone).  r may then be NULL if it is not needed, and may be x itself
  *     whether or not there is a block;
  *   stats, post_stats [rows, 2]: mean (0 for RMS) and 1 / deviation of each row for the backward pass, NULL if unwanted.
- * epsilon must be above 0. */
+ * epsilon must be above 0; rows have at most 2^24 elements and gates at most 2^30 rows (NOT_SUPPORTED beyond). */
 enum { SNB200_NORM_NONE = 0, SNB200_NORM_LAYER = 1, SNB200_NORM_RMS = 2 };
 typedef struct snb200_norm_desc {
   long long rows;

@@ -1652,6 +1652,8 @@ extern "C" int snb200_adam_group_update(snb200_handle_t h, int n, const snb200_a
       else if (t.count > 0) {
         const void* p[5] = {t.W, t.adam_vW, t.adam_sW, t.v_scale, t.s_scale};
         if (!p[k] || !t.dW) st = fail(h, SNB200_STATUS_INVALID_VALUE, "tensor %d: null pointer", i);
+        else if (t.adam_vW == t.adam_sW || t.W == t.adam_vW || t.W == t.adam_sW || t.W == t.dW)
+          st = fail(h, SNB200_STATUS_INVALID_VALUE, "tensor %d: weights, gradient and moments share memory", i);
         const size_t bytes = k >= 3 ? 4 * ((static_cast<size_t>(t.count) + kAdamBlock8 - 1) / kAdamBlock8)
                                     : static_cast<size_t>(t.count) * ((k == 0 || state_bits == 32) ? 4 : 1);
         ranges[m].begin = static_cast<const char*>(p[k]);
@@ -1683,12 +1685,20 @@ static int check_index_type(snb200_handle_t h, int index_type, const void* indic
   return 0;
 }
 
+// Sizes beyond which products of them would not fit the kernels' indices.
+static int check_embedding_sizes(snb200_handle_t h, long long tokens, int vocabulary, int dim) {
+  if (tokens < 0 || vocabulary < 1 || dim < 0)
+    return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension or empty vocabulary");
+  if (tokens > (1ll << 40) || dim > (1 << 24))
+    return fail(h, SNB200_STATUS_NOT_SUPPORTED, "%lld tokens of %d columns are more than one call takes", tokens, dim);
+  return 0;
+}
+
 extern "C" int snb200_embedding_fwd(snb200_handle_t h, int index_type, long long tokens, int vocabulary, int dim,
                                     const void* indices, float scale, const float* table, float* y) {
   int st = enter(h);
   if (st) return st;
-  if (tokens < 0 || vocabulary < 1 || dim < 0)
-    return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension or empty vocabulary");
+  if ((st = check_embedding_sizes(h, tokens, vocabulary, dim))) return st;
   if ((st = check_index_type(h, index_type, indices))) return st;
   if (tokens == 0 || dim == 0) return 0;
   if (!indices || !table || !y) return fail(h, SNB200_STATUS_INVALID_VALUE, "null pointer");
@@ -1720,7 +1730,7 @@ struct EmbeddingPlan {
   size_t pairs[2], present, crossing, counts, totals, partial, bytes;   // offsets in the scratch memory
 };
 static bool embedding_plan(long long tokens, int vocabulary, int dim, EmbeddingPlan* p) {
-  if (tokens < 0 || tokens > (1ll << 30) || vocabulary < 1 || dim < 0) return false;
+  if (tokens < 0 || tokens > (1ll << 30) || vocabulary < 1 || dim < 0 || dim > (1 << 24)) return false;
   const long long n = tokens;
   p->cluster = n <= kSortClusterTokens;
   if (p->cluster) {
@@ -1761,8 +1771,7 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
                                     void* scratch, float* dtable) {
   int st = enter(h);
   if (st) return st;
-  if (tokens < 0 || vocabulary < 1 || dim < 0)
-    return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension or empty vocabulary");
+  if ((st = check_embedding_sizes(h, tokens, vocabulary, dim))) return st;
   if ((st = check_index_type(h, index_type, indices))) return st;
   EmbeddingPlan plan;
   if (!embedding_plan(tokens, vocabulary, dim, &plan)) return fail(h, SNB200_STATUS_NOT_SUPPORTED, "more than 2^30 tokens");
@@ -1869,6 +1878,8 @@ extern "C" int snb200_embedding_bwd(snb200_handle_t h, int index_type, long long
 static int norm_check(snb200_handle_t h, const snb200_norm_desc* d, const snb200_norm_params* p) {
   if (!d || !p) return fail(h, SNB200_STATUS_INVALID_VALUE, "null descriptor or parameters");
   if (d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return fail(h, SNB200_STATUS_INVALID_VALUE, "negative dimension");
+  if (d->dim > (1 << 24) || d->gate_rows > (1 << 30))
+    return fail(h, SNB200_STATUS_NOT_SUPPORTED, "rows of %d elements, %d rows of the gate: more than one call takes", d->dim, d->gate_rows);
   const int kinds[2] = {d->norm, d->post_norm};
   for (int k = 0; k < 2; ++k)
     if (kinds[k] != SNB200_NORM_NONE && kinds[k] != SNB200_NORM_LAYER && kinds[k] != SNB200_NORM_RMS)
@@ -1947,7 +1958,7 @@ static NormPlan norm_plan(const snb200_norm_desc* d) {
   return n;
 }
 extern "C" long long snb200_residual_norm_scratch_floats(const snb200_norm_desc* d) {
-  if (!d || d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return -1;
+  if (!d || d->rows < 0 || d->dim < 0 || d->gate_rows < 0 || d->dim > (1 << 24) || d->gate_rows > (1 << 30)) return -1;
   const NormPlan n = norm_plan(d);
   const long long sums = 2 * (d->norm != SNB200_NORM_NONE) + 2 * (d->post_norm != SNB200_NORM_NONE) + (d->gate_rows == 1);
   return (sums * n.blocks + (d->gate_rows > 1 && n.pieces > 1 ? n.units : 0)) * d->dim;

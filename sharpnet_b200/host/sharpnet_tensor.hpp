@@ -387,4 +387,115 @@ class MultiheadAttention {
   std::unique_ptr<GPUTensor> scratch_;
 };
 
+// The word embedding (GPU kernels WordEmbeddingForwardPropagation / WordEmbeddingBackwardPropagation,
+// Prod/GPU/Kernels/SinglePrecision.cu:617,650) over snb200_embedding_fwd / _bwd.  x holds the word indices as floats, as
+// SharpNet's tensors do; weights and weightGradients are [vocabulary, embeddingDim] and belong to the caller, the scratch
+// memory of the backward pass to the layer.
+class EmbeddingLayer {
+ public:
+  EmbeddingLayer(int vocabularySize, int embeddingDim, float scale, int paddingIndex, GPUWrapper& wrapper)
+      : vocabulary_(vocabularySize), dim_(embeddingDim), scale_(scale), padding_(paddingIndex), wrapper_(&wrapper) {}
+  ~EmbeddingLayer() { for (void* p : scratch_) cudaFree(p); }
+  EmbeddingLayer(const EmbeddingLayer&) = delete;
+  EmbeddingLayer& operator=(const EmbeddingLayer&) = delete;
+  void ForwardPropagation(const GPUTensor& x, const GPUTensor& weights, GPUTensor& y) {
+    wrapper_->CheckStatus(snb200_embedding_fwd(wrapper_->Handle(), SNB200_INDEX_FP32, x.Count(), vocabulary_, dim_, x.Pointer(), scale_,
+                                               weights.Pointer(), y.Pointer()));
+  }
+  void BackwardPropagation(const GPUTensor& x, const GPUTensor& dy, bool accumulate, GPUTensor& weightGradients) {
+    const long long need = snb200_embedding_scratch_bytes(x.Count(), vocabulary_, dim_);
+    if (need > bytes_) {                       // kernels queued earlier may still use the smaller one: it stays
+      void* p = nullptr;
+      if (cudaMalloc(&p, static_cast<size_t>(need)) != cudaSuccess) throw std::runtime_error("cudaMalloc failed");
+      scratch_.push_back(p);
+      bytes_ = need;
+    }
+    wrapper_->CheckStatus(snb200_embedding_bwd(wrapper_->Handle(), SNB200_INDEX_FP32, x.Count(), vocabulary_, dim_, x.Pointer(), scale_,
+                                               padding_, accumulate, dy.Pointer(), scratch_.empty() ? nullptr : scratch_.back(),
+                                               weightGradients.Pointer()));
+  }
+
+ private:
+  int vocabulary_, dim_;
+  float scale_;
+  int padding_;
+  GPUWrapper* wrapper_;
+  std::vector<void*> scratch_;
+  long long bytes_ = 0;
+};
+
+// The step between two blocks: r = residualScale x + blockScale gate * post_norm(block), y = norm(r), over
+// snb200_residual_norm_fwd / _bwd.  Parameters and gradients belong to the caller (null where there is none or it is not
+// wanted); the statistics that the backward pass needs and its scratch memory to the layer.
+class ResidualNorm {
+ public:
+  struct Parameters { const GPUTensor *gamma, *beta, *post_gamma, *post_beta, *gate; };
+  struct Gradients { GPUTensor *gamma, *beta, *post_gamma, *post_beta, *gate; };
+  ResidualNorm(int dim, int norm, int postNorm, int gateRows, float residualScale, float blockScale, float epsilon, GPUWrapper& wrapper)
+      : desc_{0, dim, norm, postNorm, gateRows, residualScale, blockScale, epsilon}, wrapper_(&wrapper) {}
+  // block null: a norm alone; r may then be null, and may always be x
+  void ForwardPropagation(const GPUTensor& x, const GPUTensor* block, const Parameters& p, GPUTensor* r, GPUTensor* y) {
+    desc_.rows = x.Count() / desc_.dim;
+    const snb200_norm_params params = Pack(p);
+    wrapper_->CheckStatus(snb200_residual_norm_fwd(wrapper_->Handle(), &desc_, &params, x.Pointer(), Ptr(block), Ptr(r), Ptr(y),
+                                                   Room(stats_, 2 * desc_.rows), Room(post_stats_, 2 * desc_.rows)));
+  }
+  void BackwardPropagation(const GPUTensor& r, const GPUTensor* block, const GPUTensor* dy, const GPUTensor* dr, const Parameters& p,
+                           const Gradients& g, GPUTensor* dx, GPUTensor* dblock) {
+    desc_.rows = r.Count() / desc_.dim;
+    const snb200_norm_params params = Pack(p);
+    const snb200_norm_gradients grads = {Ptr(g.gamma), Ptr(g.beta), Ptr(g.post_gamma), Ptr(g.post_beta), Ptr(g.gate)};
+    wrapper_->CheckStatus(snb200_residual_norm_bwd(wrapper_->Handle(), &desc_, &params, r.Pointer(), Ptr(block), Ptr(dy), Ptr(dr),
+                                                   Room(stats_, 2 * desc_.rows), Room(post_stats_, 2 * desc_.rows),
+                                                   Room(scratch_, snb200_residual_norm_scratch_floats(&desc_)), Ptr(dx), Ptr(dblock), &grads));
+  }
+
+ private:
+  typedef std::vector<std::unique_ptr<GPUTensor>> Buffers;     // the last one is in use; queued kernels may still use the others
+  static float* Ptr(const GPUTensor* t) { return t ? t->Pointer() : nullptr; }
+  static snb200_norm_params Pack(const Parameters& p) { return {Ptr(p.gamma), Ptr(p.beta), Ptr(p.post_gamma), Ptr(p.post_beta), Ptr(p.gate)}; }
+  float* Room(Buffers& buffers, long long floats) {
+    if (buffers.empty() || buffers.back()->Count() < floats)
+      buffers.emplace_back(new GPUTensor({static_cast<int>((floats + 3) / 4), 4}, nullptr, *wrapper_));
+    return buffers.back()->Pointer();
+  }
+  snb200_norm_desc desc_;
+  GPUWrapper* wrapper_;
+  Buffers stats_, post_stats_, scratch_;
+};
+
+// Adam / AdamW over all parameter tensors as one launch, with moments in 32 or 8 bits (the loop over the layers'
+// Adam.UpdateWeights, Prod/Optimizers/Adam.cs:59-72); decay: the factor of the weight decay for that tensor.
+class AdamGroup {
+ public:
+  struct Tensor { GPUTensor* weights; const GPUTensor* weightGradients; double decay; };
+  AdamGroup(const std::vector<Tensor>& tensors, double beta1, double beta2, double eps, double weightDecay, int stateBits, GPUWrapper& wrapper)
+      : beta1_(beta1), beta2_(beta2), eps_(eps), decay_(weightDecay), bits_(stateBits), wrapper_(&wrapper) {
+    for (const Tensor& t : tensors) {
+      const long long n = t.weights->Count(), blocks = (n + 255) / 256;
+      const long long moment = bits_ == 8 ? (n + 3) / 4 : n;                 // floats that hold one moment
+      auto zeros = [this](long long floats) {
+        state_.emplace_back(new GPUTensor({static_cast<int>(floats)}, nullptr, *wrapper_));
+        return state_.back()->Pointer();
+      };
+      snb200_adam_tensor a = {n, t.weightGradients->Pointer(), t.weights->Pointer(), zeros(moment), zeros(moment), nullptr, nullptr, t.decay};
+      if (bits_ == 8) { a.v_scale = zeros(blocks); a.s_scale = zeros(blocks); }
+      table_.push_back(a);
+    }
+  }
+  void UpdateWeights(double learningRate, double maxLearningRate) {
+    ++timestep_;
+    wrapper_->CheckStatus(snb200_adam_group_update(wrapper_->Handle(), static_cast<int>(table_.size()), table_.data(), bits_, learningRate,
+                                                   beta1_, beta2_, eps_, learningRate / maxLearningRate * decay_, timestep_,
+                                                   static_cast<unsigned>(timestep_)));
+  }
+
+ private:
+  double beta1_, beta2_, eps_, decay_;
+  int bits_, timestep_ = 0;
+  GPUWrapper* wrapper_;
+  std::vector<std::unique_ptr<GPUTensor>> state_;
+  std::vector<snb200_adam_tensor> table_;
+};
+
 }  // namespace SharpNet

@@ -216,6 +216,10 @@ def test_refusals(wrapper):
             table = _table(up, [1, 1])
             setattr(table[1], field, getattr(table[0], field) + offset)
             assert call(table) == 7 and b"share memory" in wrapper.lib.snb200_last_error_string(wrapper.handle), field
+    for field, other in (("adam_sW", "adam_vW"), ("adam_vW", "W"), ("adam_sW", "W"), ("W", "dW")):
+        table = _table(up, [1, 1])
+        setattr(table[0], field, getattr(table[0], other))
+        assert call(table) == 7, (field, other)
     table = (_capi.AdamTensor * 2)(good[1], good[0])                            # descending order is no overlap
     assert call(table) == 0
     for u, h in zip(up, host):

@@ -231,6 +231,8 @@ def test_refusals(wrapper):
     assert bwd(h, 0, 4, 4, 4, p, 1.0, -1, 0, p, p, None) == 7
     assert bwd(h, 0, 4, 4, 4, p, 1.0, -1, 0, p, p + 4, p) == 7                     # scratch alignment
     assert bwd(h, 0, (1 << 30) + 1, 4, 4, p, 1.0, -1, 0, p, p, p) == 15
+    assert fwd(h, 0, 4, 4, (1 << 24) + 1, p, 1.0, p, p) == 15 and fwd(h, 0, 1 << 62, 4, 4, p, 1.0, p, p) == 15
+    assert bwd(h, 0, 4, 4, (1 << 24) + 1, p, 1.0, -1, 0, p, p, p) == 15 and lib.snb200_embedding_scratch_bytes(4, 4, (1 << 24) + 1) == -1
     assert fwd(h, 0, 0, 4, 4, None, 1.0, None, None) == 0 and fwd(h, 0, 4, 4, 0, None, 1.0, None, None) == 0
     assert not t.cpu().numpy().any()
 

@@ -367,6 +367,8 @@ def test_refusals(wrapper):
         assert call(_desc(4, 4, "layer", "none", 3, 1, 1), P(gate=q)) == 7 and call(_desc(4, 4, "layer", "none", 8, 1, 1), P(gate=q)) == 7
         assert call(_desc(4, 4, "layer", "none", 1, 1, 1)) == 7 and call(_desc(4, 4, "layer", "none", 0, 1, 1), P(gate=q)) == 7
         assert call(_desc(4, 4, "none", "rms", 0, 1, 1), P(gamma=q)) == 7 and call(_desc(4, 4, "rms", "none", 0, 1, 1), P(post_beta=q)) == 7
+        assert call(_desc(4, (1 << 24) + 1, "layer", "none", 0, 1, 1)) == 15
+        assert call(_desc(1 << 31, 4, "layer", "none", (1 << 30) + 1, 1, 1), P(gate=q)) == 15
         assert lib.snb200_last_error_string(h)
     layer = _desc(4, 4, "layer", "none", 0, 1, 1)
     assert fwd(layer, x=None) == 7 and fwd(layer, y=None) == 7 and fwd(layer, r=None) == 7
