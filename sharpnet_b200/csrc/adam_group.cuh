@@ -29,7 +29,8 @@ struct AdamTensor {
   unsigned ordinal_vec;   // the tensor's place in the caller's list << 1, and whether its pointers allow vector accesses
 };
 // N tensors and the number of the first work item of each.  A kernel takes at most 32764 bytes of parameters: 448
-// tensors fill 30472; the small table keeps a small model's launch from copying as much.
+// tensors fill 30472.  Up to 32 tensors take a small one: the launch copies the whole parameter, and a step of 16 tensors
+// costs the host 5.8 us instead of 8.6 (the device the same 4.5).
 constexpr int kAdamMaxTensors = 448;
 template <int N> struct AdamTable {
   int n;
@@ -55,6 +56,7 @@ __device__ __forceinline__ void adam32_one(const AdamCoefficients& c, float wd, 
   w = __fsub_rn(w, __fmaf_rn(wd, w, __fdiv_rn(__fmul_rn(c.factor, v), __fadd_rn(__fsqrt_rn(s), c.eps))));
 }
 
+// Bound by memory: 28 bytes an element, 57.7 us for 12.6 M of them (6.1 TB/s).
 template <int N>
 static __global__ void __launch_bounds__(kAdamThreads)
 adam_group32_kernel(const __grid_constant__ AdamTable<N> table, const AdamCoefficients c) {
@@ -166,7 +168,7 @@ __device__ __forceinline__ void copy_async_4(void* smem, const void* global) {
 // elements go through the packed 32-bit arithmetic; the quotient of the weight's step, which no state depends on, is a
 // product with the approximate reciprocal (2 ulp); the rounding below 2^-6, which few elements need, sits behind a branch.
 // A block's elements are copied into shared memory slots of the thread that updates them while the block before them is
-// updated.
+// updated (185 M parameters: 617 us without, 498 with two blocks an item; 6.0 TB/s).
 template <int N>
 static __global__ void __launch_bounds__(kAdamThreads, 4)
 adam_group8_kernel(const __grid_constant__ AdamTable<N> table, const AdamCoefficients c, const unsigned seed) {

@@ -36,7 +36,7 @@ __device__ __forceinline__ int load_index(const void* indices, int index_type, l
 
 // ---------------------------------------------------------------- forward
 // Block of bx x by threads: bx consecutive vectors of a row, by rows side by side, TOKENS rows per thread one after the
-// other with their loads in flight together.
+// other with their loads in flight together.  Bound by memory: 16384 rows of 1024 take 17.0 us (5.3 TB/s).
 template <int VEC, int TOKENS>
 static __global__ void __launch_bounds__(256)
 embedding_fwd_kernel(const void* __restrict__ indices, int index_type, long long tokens, int vocab, int row_vecs, float scale,
@@ -186,6 +186,7 @@ __device__ __forceinline__ uint2 sort_pair(const SortPass& p, int i) {
 
 // The words that a block's tokens name, gathered in shared memory (a frequent word asks for its bit thousands of times) and
 // handed over once, where the vocabulary's bits fit; by themselves, and only where the bit is not there yet, where not.
+// (262144 tokens of 131072 words: the counting launch takes 44 us with an atomic a token, 7 so.)
 constexpr int kPresentWords = 4096;                    // 131072 words: 16 KB
 __device__ __forceinline__ void present_mark(const SortPass& p, unsigned* bits, unsigned word) {
   if (word >= static_cast<unsigned>(p.vocab)) return;
@@ -353,7 +354,8 @@ sort_scatter_kernel(const SortPass p, const ZeroRows z) {
 // of its warps' strips, the blocks read each other's counts through distributed shared memory, and the pairs go to their
 // places in the blocks' shared memory, the last pass's to global memory.  The other clusters of the launch clear the
 // gradient meanwhile, all of it: the rows that are summed later are few here (at most a row a token), and waiting for the
-// list of those that are not would cost more than writing them twice.
+// list of those that are not would cost more than writing them twice.  Bound by the latency of its barriers: 8 us for 4999
+// tokens, hidden behind the clearing of a table of 134 MB (20 us).
 constexpr int kSortCluster = 8;
 constexpr int kSortClusterTile = kSortClusterTokens / kSortCluster;
 struct SortAll {
@@ -456,7 +458,8 @@ __device__ __forceinline__ void store_word(const WordSums& p, unsigned word, int
 
 // A warp a chunk and slab.  U rows are in flight per lane; with ACCUMULATE the row that a word's sum is added to is fetched
 // with the word's first row, not when the sum is done (in a long tail of words that occur once that would be one memory
-// latency a row).
+// latency a row).  Bound by memory on a long batch: 262144 rows of 1024 take 200 us (1.2 GB at 6.1 TB/s); by its waves of
+// blocks on a short one (16384 rows: 16 to 18 us for 97 MB, at four blocks a SM; 22 at three).
 template <int VEC, bool ACCUMULATE>
 static __global__ void __launch_bounds__(256, VEC == 4 && !ACCUMULATE ? 4 : 2)
 word_sums_kernel(const WordSums p) {
@@ -521,7 +524,8 @@ word_sums_kernel(const WordSums p) {
 
 // The words that cross chunks.  (The order of the list does not matter: each entry is a word of its own.)  A warp takes a
 // slab of a word and adds its partial sums in chunk order; where there are many, the block's eight warps add up eight runs
-// of them, and their sums are added in order.
+// of them, and their sums are added in order.  Bound by latency: 10 us for the 1300 words that cross in 262144 tokens (33 us
+// with a block a word, whose neighbours in the list were slabs of the same word).
 template <int VEC>
 static __global__ void __launch_bounds__(256)
 word_join_kernel(const WordSums p) {
