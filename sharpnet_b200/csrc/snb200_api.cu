@@ -1953,7 +1953,8 @@ static NormPlan norm_plan(const snb200_norm_desc* d) {
   long long pieces = 1, best = 0;
   for (int waves = 1; waves <= 4; ++waves) {
     long long k = waves * all / groups;
-    k = k > per ? per : k < 1 ? 1 : k;
+    if (k > per) k = per;
+    if (k < 1) k = 1;                                // (no rows: one empty piece)
     const long long line = (groups * k + all - 1) / all * ((per + k - 1) / k + 1);
     if (waves == 1 || line < best) { pieces = k; best = line; }
   }
